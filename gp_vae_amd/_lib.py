@@ -9,9 +9,12 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libgpvae_hip.so")
+LOWBIT_PATH = os.path.join(_HERE, "libgpvae_lowbit.so")  # include/gpvae_lowbit.h
 
 F32, F64 = 0, 1
 ABI_VERSION = 2  # include/gpvae.h GPVAE_ABI_VERSION
+LB_F32, LB_BF16, LB_F16 = 0, 2, 3  # include/gpvae_lowbit.h
+LOWBIT_ABI_VERSION = 1
 POTRF_ZERO_UPPER, POTRF_NAN_ON_FAIL, POTRF_SHARE_CHIP = 1, 2, 4
 
 
@@ -81,7 +84,28 @@ SIGNATURES = {
     "gpvae_decoder_vjp_static": (_i, [_vp, _i, _i64, _i64, _i, _i, _i, _vp, _vp, _vp, _vp]),
 }
 
+# name -> (restype, argtypes); must list every symbol include/gpvae_lowbit.h declares
+LOWBIT_SIGNATURES = {
+    "gpvae_lowbit_abi_version": (_i, []),
+    "gpvae_lowbit_last_error": (C.c_char_p, []),
+    "gpvae_w4_code_bytes": (_i64, [_i64, _i64]),
+    "gpvae_w4_exp_bytes": (_i64, [_i64, _i64]),
+    "gpvae_quant_w4": (_i, [_vp, _i, _i64, _i64, _vp, _i64, _vp, _vp]),
+    "gpvae_load_w4": (_i, [_vp, _i, _i64, _i64, _vp, _vp, _vp, _i64]),
+    "gpvae_dense_w4_workspace_bytes": (_i64, [_i, _i64, _i64, _i64]),
+    "gpvae_dense_w4": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _i, _vp, _i64, _vp]),
+    "gpvae_dense_vjp_w4_workspace_bytes": (_i64, [_i, _i64, _i64, _i64]),
+    "gpvae_dense_vjp_w4": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "gpvae_q8_code_bytes": (_i64, [_i64, _i64]),
+    "gpvae_q8_exp_bytes": (_i64, [_i64, _i64]),
+    "gpvae_store_q8": (_i, [_vp, _i, _i64, _i64, _vp, _i64, _i, _vp, _i64, _vp, _vp]),
+    "gpvae_load_q8": (_i, [_vp, _i, _i64, _i64, _i, _vp, _vp, _vp, _i64]),
+    "gpvae_dense_grads_q8_workspace_bytes": (_i64, [_i, _i64, _i64, _i64]),
+    "gpvae_dense_grads_q8": (_i, [_vp, _i, _i64, _i64, _i64, _i, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp]),
+}
+
 _lib = None
+_lowbit = None
 
 
 def load():
@@ -108,4 +132,31 @@ def load():
 def check(rc, what):
     if rc != 0:
         msg = load().gpvae_last_error()
+        raise GpvaeError("%s failed (rc=%d): %s" % (what, rc, msg.decode() if msg else ""))
+
+
+def load_lowbit():
+    """The ctypes handle of libgpvae_lowbit.so (include/gpvae_lowbit.h), loaded once; raises GpvaeError if it is absent."""
+    global _lowbit
+    if _lowbit is not None:
+        return _lowbit
+    if not os.path.exists(LOWBIT_PATH):
+        raise GpvaeError(
+            "libgpvae_lowbit.so not found at %s: the HIP library is required (no CPU fallback). "
+            "Build it with `make -C gp_vae_amd/csrc` or __graft_entry__.build()." % LOWBIT_PATH)
+    lib = C.CDLL(LOWBIT_PATH)
+    for name, (res, args) in LOWBIT_SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype = res
+        fn.argtypes = args
+    if lib.gpvae_lowbit_abi_version() != LOWBIT_ABI_VERSION:
+        raise GpvaeError("libgpvae_lowbit.so reports ABI version %d, this binding was written for %d — rebuild with "
+                         "`make -C gp_vae_amd/csrc`" % (lib.gpvae_lowbit_abi_version(), LOWBIT_ABI_VERSION))
+    _lowbit = lib
+    return lib
+
+
+def check_lowbit(rc, what):
+    if rc != 0:
+        msg = load_lowbit().gpvae_lowbit_last_error()
         raise GpvaeError("%s failed (rc=%d): %s" % (what, rc, msg.decode() if msg else ""))

@@ -1,0 +1,177 @@
+// w4.hip — dense layers with weights in 4 bits: quantiser, reader, the product and the transposed product.
+#include "lowbit.hpp"
+
+namespace gpvae_lb {
+
+// One thread per tile of 8 x 8.
+template <typename T>
+__global__ __launch_bounds__(256) void quant_w4_kernel(int64_t K, int64_t N, const T *__restrict__ W, int64_t ldw,
+                                                       uint32_t *__restrict__ codes, uint8_t *__restrict__ exps) {
+  const int64_t Np = w4_np(N), nt = Np / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= w4_kb(K) * 4 * nt) return;
+  const int64_t t = id % nt, kt = id / nt, k0 = kt * 8, n0 = t * 8;
+  float amax = 0.0f;
+  bool bad = false;
+  for (int i = 0; i < 8; ++i)
+    for (int c = 0; c < 8; ++c)
+      if (k0 + i < K && n0 + c < N) {
+        const float a = fabsf(to_f32(W[(k0 + i) * ldw + n0 + c]));
+        bad |= !(a <= 3.402823466e+38f);
+        amax = fmaxf(amax, a);
+      }
+  const int eb = bad ? 255 : tile_exp_byte<6, 2, -125>(amax);
+  exps[(kt / 4 * nt + t) * 4 + kt % 4] = (uint8_t)eb;
+  for (int c = 0; c < 8; ++c) {
+    uint32_t w = 0;
+    for (int i = 0; i < 8; ++i)
+      if (k0 + i < K && n0 + c < N && !bad) w |= e2m1_code(unscale<6>(to_f32(W[(k0 + i) * ldw + n0 + c]), eb)) << (4 * i);
+    codes[((kt / 4) * Np + n0 + c) * 4 + kt % 4] = w;
+  }
+}
+
+// value of row k, column n
+__device__ __forceinline__ float w4_value(const uint32_t *codes, const uint8_t *exps, int64_t Np, int64_t k, int64_t n) {
+  const int64_t kb = k / 32;
+  const int j = (int)(k / 8) % 4, i = (int)(k % 8);
+  const uint32_t w = codes[(kb * Np + n) * 4 + j] >> (4 * i);
+  const float s = scale_of(exps[(kb * (Np / 8) + n / 8) * 4 + j]);
+  return bf_lo(w4_pair<0>(w, s));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void load_w4_kernel(int64_t K, int64_t N, const uint32_t *__restrict__ codes,
+                                                      const uint8_t *__restrict__ exps, T *__restrict__ out, int64_t ldo) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, Np = w4_np(N);
+  if (n >= N) return;
+  for (int64_t k = blockIdx.y; k < K; k += gridDim.y) out[k * ldo + n] = from_f32<T>(w4_value(codes, exps, Np, k, n));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void dense_w4_kernel(int64_t M, int64_t K, int64_t N, const T *__restrict__ X, int64_t ldx,
+                                                       const uint32_t *__restrict__ codes, const uint8_t *__restrict__ exps,
+                                                       const T *__restrict__ bias, int relu, T *__restrict__ Y, int64_t ldy) {
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, Np = w4_np(N);
+  if (n >= N) return;
+  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+    float a = 0.0f;
+    for (int64_t k = 0; k < K; ++k) a = fmaf(to_f32(X[m * ldx + k]), w4_value(codes, exps, Np, k, n), a);
+    if (bias) a += to_f32(bias[n]);
+    if (relu) a = a < 0.0f ? 0.0f : a;
+    Y[m * ldy + n] = from_f32<T>(a);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void dense_vjp_w4_kernel(int64_t M, int64_t K, int64_t N, const T *__restrict__ dY,
+                                                           int64_t lddy, const uint32_t *__restrict__ codes,
+                                                           const uint8_t *__restrict__ exps, const uint8_t *__restrict__ act,
+                                                           T *__restrict__ dX, int64_t lddx) {
+  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, Np = w4_np(N);
+  if (k >= K) return;
+  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+    float a = 0.0f;
+    for (int64_t n = 0; n < N; ++n) a = fmaf(to_f32(dY[m * lddy + n]), w4_value(codes, exps, Np, k, n), a);
+    if (act && act[((m / 8) * q8_kp(K) + k) * 8 + m % 8] == 0) a = 0.0f;
+    dX[m * lddx + k] = from_f32<T>(a);
+  }
+}
+
+static int check_w4(const char *fn, int dtype, int64_t K, int64_t N, int kn_arg) {
+  LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
+  LB_REQUIRE(K >= 1 && K <= (1 << 30), kn_arg, "%s: K must lie in [1, 2^30] (got %lld)", fn, (long long)K);
+  LB_REQUIRE(N >= 1 && N <= (1 << 30), kn_arg + 1, "%s: N must lie in [1, 2^30] (got %lld)", fn, (long long)N);
+  return 0;
+}
+
+}  // namespace gpvae_lb
+
+using namespace gpvae_lb;
+
+extern "C" int gpvae_quant_w4(void *stream, int dtype, int64_t K, int64_t N, const void *W, int64_t ldw, void *codes,
+                              void *exps) {
+  const char *fn = "gpvae_quant_w4";
+  if (const int rc = check_w4(fn, dtype, K, N, 3)) return rc;
+  LB_REQUIRE(W, 5, "%s: W is NULL", fn);
+  LB_REQUIRE(ldw >= N, 6, "%s: ldw < N", fn);
+  LB_REQUIRE(codes && aligned16(codes), 7, "%s: codes must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(exps && aligned16(exps), 8, "%s: exps must be a 16-byte aligned device pointer", fn);
+  const int64_t tiles = w4_kb(K) * 4 * (w4_np(N) / 8);
+  LB_REQUIRE(cdiv(tiles, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+#define GO(T)                                                                                                         \
+  hipLaunchKernelGGL(quant_w4_kernel<T>, dim3((unsigned)cdiv(tiles, 256)), dim3(256), 0, (hipStream_t)stream, K, N,  \
+                     (const T *)W, ldw, (uint32_t *)codes, (uint8_t *)exps)
+  LB_BY_DTYPE(dtype, GO);
+#undef GO
+  LB_CHECK_LAUNCH(fn);
+  return 0;
+}
+
+extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, const void *codes, const void *exps, void *out,
+                             int64_t ldo) {
+  const char *fn = "gpvae_load_w4";
+  if (const int rc = check_w4(fn, dtype, K, N, 3)) return rc;
+  LB_REQUIRE(codes && aligned16(codes), 5, "%s: codes must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(exps && aligned16(exps), 6, "%s: exps must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(out, 7, "%s: out is NULL", fn);
+  LB_REQUIRE(ldo >= N, 8, "%s: ldo < N", fn);
+  const dim3 grid((unsigned)cdiv(N, 256), (unsigned)(K < 65535 ? K : 65535));
+#define GO(T)                                                                                                     \
+  hipLaunchKernelGGL(load_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, K, N, (const uint32_t *)codes, \
+                     (const uint8_t *)exps, (T *)out, ldo)
+  LB_BY_DTYPE(dtype, GO);
+#undef GO
+  LB_CHECK_LAUNCH(fn);
+  return 0;
+}
+
+extern "C" int64_t gpvae_dense_w4_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
+extern "C" int64_t gpvae_dense_vjp_w4_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
+
+extern "C" int gpvae_dense_w4(void *stream, int dtype, int64_t M, int64_t K, int64_t N, const void *X, int64_t ldx,
+                              const void *codes, const void *exps, const void *bias, int relu, void *Y, int64_t ldy,
+                              void *work) {
+  const char *fn = "gpvae_dense_w4";
+  LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
+  LB_REQUIRE(M >= 0 && M <= (1 << 30), 3, "%s: M must lie in [0, 2^30] (got %lld)", fn, (long long)M);
+  if (const int rc = check_w4(fn, dtype, K, N, 4)) return rc;
+  if (M == 0) return 0;
+  LB_REQUIRE(X, 6, "%s: X is NULL", fn);
+  LB_REQUIRE(ldx >= K, 7, "%s: ldx < K", fn);
+  LB_REQUIRE(codes && aligned16(codes), 8, "%s: codes must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(exps && aligned16(exps), 9, "%s: exps must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(Y && Y != X, 12, "%s: Y is NULL or X", fn);
+  LB_REQUIRE(ldy >= N, 13, "%s: ldy < N", fn);
+  const dim3 grid((unsigned)cdiv(N, 256), (unsigned)(M < 65535 ? M : 65535));
+#define GO(T)                                                                                                              \
+  hipLaunchKernelGGL(dense_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, M, K, N, (const T *)X, ldx,            \
+                     (const uint32_t *)codes, (const uint8_t *)exps, (const T *)bias, relu, (T *)Y, ldy)
+  LB_BY_DTYPE(dtype, GO);
+#undef GO
+  LB_CHECK_LAUNCH(fn);
+  return 0;
+}
+
+extern "C" int gpvae_dense_vjp_w4(void *stream, int dtype, int64_t M, int64_t K, int64_t N, const void *dY, int64_t lddy,
+                                  const void *codes, const void *exps, const void *act_codes, void *dX, int64_t lddx,
+                                  void *work) {
+  const char *fn = "gpvae_dense_vjp_w4";
+  LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
+  LB_REQUIRE(M >= 0 && M <= (1 << 30), 3, "%s: M must lie in [0, 2^30] (got %lld)", fn, (long long)M);
+  if (const int rc = check_w4(fn, dtype, K, N, 4)) return rc;
+  if (M == 0) return 0;
+  LB_REQUIRE(dY, 6, "%s: dY is NULL", fn);
+  LB_REQUIRE(lddy >= N, 7, "%s: lddy < N", fn);
+  LB_REQUIRE(codes && aligned16(codes), 8, "%s: codes must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(exps && aligned16(exps), 9, "%s: exps must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(!act_codes || aligned16(act_codes), 10, "%s: act_codes must be 16-byte aligned", fn);
+  LB_REQUIRE(dX && dX != dY, 11, "%s: dX is NULL or dY", fn);
+  LB_REQUIRE(lddx >= K, 12, "%s: lddx < K", fn);
+  const dim3 grid((unsigned)cdiv(K, 256), (unsigned)(M < 65535 ? M : 65535));
+#define GO(T)                                                                                                            \
+  hipLaunchKernelGGL(dense_vjp_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, M, K, N, (const T *)dY, lddy,    \
+                     (const uint32_t *)codes, (const uint8_t *)exps, (const uint8_t *)act_codes, (T *)dX, lddx)
+  LB_BY_DTYPE(dtype, GO);
+#undef GO
+  LB_CHECK_LAUNCH(fn);
+  return 0;
+}

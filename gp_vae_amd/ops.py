@@ -9,7 +9,8 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import F32, F64, GpvaeError, POTRF_NAN_ON_FAIL, POTRF_SHARE_CHIP, POTRF_ZERO_UPPER, check
+from ._lib import (F32, F64, LB_BF16, LB_F16, LB_F32, GpvaeError, POTRF_NAN_ON_FAIL, POTRF_SHARE_CHIP, POTRF_ZERO_UPPER,
+                   check, check_lowbit)
 
 _DT = {torch.float32: F32, torch.float64: F64}
 
@@ -692,3 +693,224 @@ def decoder_vjp_static(dec_params, Z, dF, h0, h1, out=None):
     check(_lib.load().gpvae_decoder_vjp_static(_stream(), _dt(Z), C_, n, h0, h1, z, _p(dec_params), _p(Z),
                                                _p(dF), _p(dZ)), "gpvae_decoder_vjp_static")
     return dZ
+
+
+# ---- dense layers with weights in 4 bits, activation checkpoints in 8 bits (include/gpvae_lowbit.h) -------------
+# The arguments may live on any device: the launch goes to the current stream of THEIR device.
+_LB_DT = {torch.float32: LB_F32, torch.bfloat16: LB_BF16, torch.float16: LB_F16}
+
+
+def _lb_dt(what, t):
+    try:
+        return _LB_DT[t.dtype]
+    except KeyError:
+        raise GpvaeError("%s: unsupported dtype %s (float32/bfloat16/float16 only)" % (what, t.dtype))
+
+
+def _lb_mat(what, name, t, cols=None, rows=None):
+    """A [rows, cols] device matrix the library can read (unit column stride, rows apart), copied if need be."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 2:
+        raise GpvaeError("%s: %s must be a 2-D tensor" % (what, name))
+    _dev(t)
+    if (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
+        raise GpvaeError("%s: %s must be [%s, %s]; got %s" % (what, name, "rows" if rows is None else rows,
+                                                              "columns" if cols is None else cols, tuple(t.shape)))
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+        if t.stride(1) != 1 or t.stride(0) < t.shape[1]:  # torch calls a one-row or one-column view contiguous as it is
+            t = torch.empty_strided(t.shape, (t.shape[1], 1), dtype=t.dtype, device=t.device).copy_(t)
+    return t
+
+
+def _lb_out(what, out, shape, like, src):
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if (not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != like.dtype
+            or out.device != like.device or out.stride(1) != 1 or out.stride(0) < shape[1]):
+        raise GpvaeError("%s: out must be a %s tensor %s on %s with unit column stride and rows that do not overlap"
+                         % (what, like.dtype, tuple(shape), like.device))
+    if shape[0] and src is not None and out.data_ptr() == src.data_ptr():
+        raise GpvaeError("%s: out must not be the input" % what)
+    return out
+
+
+def _lb_same(what, dev, *ts):
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise GpvaeError("%s: operands on %s and %s" % (what, dev, t.device))
+
+
+def _lb_call(what, dev, fn, *args):
+    if dev.index == torch.cuda.current_device():
+        rc = fn(C.c_void_p(torch.cuda.current_stream().cuda_stream), *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(C.c_void_p(torch.cuda.current_stream().cuda_stream), *args)
+    if rc:
+        check_lowbit(rc, what)
+
+
+def _lb_work(nbytes, dev):
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
+
+
+class W4:
+    """Weights [K, N] of a dense layer in 4 bits: `codes` int32 [ceil(K/32), Np, 4] and `exps` uint8
+    [ceil(K/32), Np/8, 4] with Np = N rounded up to 32 (layout: include/gpvae_lowbit.h).  Made by quant_w4, or from
+    arrays of that layout."""
+
+    __slots__ = ("codes", "exps", "K", "N")
+
+    def __init__(self, codes, exps, K, N):
+        K, N = int(K), int(N)
+        kb, np_ = (K + 31) // 32, (N + 31) // 32 * 32
+        if K < 1 or N < 1 or codes.shape != (kb, np_, 4) or exps.shape != (kb, np_ // 8, 4):
+            raise GpvaeError("W4: codes must be [%d, %d, 4] and exps [%d, %d, 4] for K = %d, N = %d (both >= 1); got %s, %s"
+                             % (kb, np_, kb, np_ // 8, K, N, tuple(codes.shape), tuple(exps.shape)))
+        if codes.dtype != torch.int32 or exps.dtype != torch.uint8 or not (codes.is_contiguous() and exps.is_contiguous()):
+            raise GpvaeError("W4: codes must be contiguous int32, exps contiguous uint8")
+        if codes.device != exps.device:
+            raise GpvaeError("W4: codes on %s, exps on %s" % (codes.device, exps.device))
+        self.codes, self.exps, self.K, self.N = codes, exps, K, N
+
+
+class Q8:
+    """Checkpoint of a matrix [M, K] in 8 bits: `codes` uint8 [ceil(M/8), Kp, 8] and `exps` uint8 [ceil(M/8), Kp/8] with
+    Kp = K rounded up to 32 (layout: include/gpvae_lowbit.h); relu: stored after a ReLU (codes 0 .. 255 that carry its mask).
+    Made by store_q8, or from arrays of that layout."""
+
+    __slots__ = ("codes", "exps", "M", "K", "relu")
+
+    def __init__(self, codes, exps, M, K, relu=False):
+        M, K = int(M), int(K)
+        mb, kp = (M + 7) // 8, (K + 31) // 32 * 32
+        if M < 0 or K < 1 or codes.shape != (mb, kp, 8) or exps.shape != (mb, kp // 8):
+            raise GpvaeError("Q8: codes must be [%d, %d, 8] and exps [%d, %d] for M = %d, K = %d (K >= 1); got %s, %s"
+                             % (mb, kp, mb, kp // 8, M, K, tuple(codes.shape), tuple(exps.shape)))
+        if codes.dtype != torch.uint8 or exps.dtype != torch.uint8 or not (codes.is_contiguous() and exps.is_contiguous()):
+            raise GpvaeError("Q8: codes and exps must be contiguous uint8")
+        if codes.device != exps.device:
+            raise GpvaeError("Q8: codes on %s, exps on %s" % (codes.device, exps.device))
+        self.codes, self.exps, self.M, self.K, self.relu = codes, exps, M, K, bool(relu)
+
+
+def quant_w4(W):
+    """Weights W [K, N] (stax layout: y = x W + b; float32, bfloat16 or float16) -> :class:`W4`: E2M1 values times one power of
+    two per 8 x 8 tile, 4.125 bits a weight.  A tile with an infinity or a NaN reads as NaN."""
+    W = _lb_mat("quant_w4", "W", W)
+    K, N = W.shape
+    dt = _lb_dt("quant_w4", W)
+    if K < 1 or N < 1:
+        raise GpvaeError("quant_w4: W must not be empty; got %s" % (tuple(W.shape),))
+    kb, np_ = (K + 31) // 32, (N + 31) // 32 * 32
+    codes = torch.empty((kb, np_, 4), dtype=torch.int32, device=W.device)
+    exps = torch.empty((kb, np_ // 8, 4), dtype=torch.uint8, device=W.device)
+    _lb_call("gpvae_quant_w4", W.device, _lib.load_lowbit().gpvae_quant_w4, dt, K, N, _p(W), W.stride(0), _p(codes), _p(exps))
+    return W4(codes, exps, K, N)
+
+
+def load_w4(w4, dtype=torch.float32):
+    """The weights [K, N] the codes stand for (exact in float32 and bfloat16)."""
+    _dev(w4.codes)
+    out = torch.empty((w4.K, w4.N), dtype=dtype, device=w4.codes.device)
+    _lb_call("gpvae_load_w4", out.device, _lib.load_lowbit().gpvae_load_w4, _lb_dt("load_w4", out), w4.K, w4.N, _p(w4.codes),
+             _p(w4.exps), _p(out), w4.N)
+    return out
+
+
+def dense_w4(X, w4, bias=None, relu=False, out=None):
+    """Y = X W + bias [M, N] (relu: max(., 0)) for X [M, K] and weights in 4 bits, for one row or thousands; X float32,
+    bfloat16 or float16, bias [N] and Y of its type, sums in float32."""
+    X = _lb_mat("dense_w4", "X", X, cols=w4.K)
+    dt, dev, M = _lb_dt("dense_w4", X), X.device, X.shape[0]
+    if bias is not None:
+        if bias.shape != (w4.N,) or bias.dtype != X.dtype:
+            raise GpvaeError("dense_w4: bias must be a %s tensor [%d]" % (X.dtype, w4.N))
+        bias = bias.contiguous()
+    _lb_same("dense_w4", dev, w4.codes, bias)
+    Y = _lb_out("dense_w4", out, (M, w4.N), X, X)
+    lib = _lib.load_lowbit()
+    work = _lb_work(lib.gpvae_dense_w4_workspace_bytes(dt, M, w4.K, w4.N), dev)
+    _lb_call("gpvae_dense_w4", dev, lib.gpvae_dense_w4, dt, M, w4.K, w4.N, _p(X), X.stride(0), _p(w4.codes), _p(w4.exps),
+             _p(bias), int(bool(relu)), _p(Y), Y.stride(0), _p(work))
+    return Y
+
+
+def dense_vjp_w4(dY, w4, act=None, out=None):
+    """dX = dY W^T [M, K] for dY [M, N] and weights in 4 bits.  act: the :class:`Q8` checkpoint (relu=True) of the layer's
+    input; dX is then also multiplied by its mask (input > 0), i.e. it is the gradient before the ReLU that made the input."""
+    dY = _lb_mat("dense_vjp_w4", "dY", dY, cols=w4.N)
+    dt, dev, M = _lb_dt("dense_vjp_w4", dY), dY.device, dY.shape[0]
+    if act is not None:
+        if not act.relu:
+            raise GpvaeError("dense_vjp_w4: act must be a checkpoint stored with relu=True (its codes carry the mask)")
+        if (act.M, act.K) != (M, w4.K):
+            raise GpvaeError("dense_vjp_w4: act must be a checkpoint of [%d, %d]; got [%d, %d]" % (M, w4.K, act.M, act.K))
+    _lb_same("dense_vjp_w4", dev, w4.codes, None if act is None else act.codes)
+    dX = _lb_out("dense_vjp_w4", out, (M, w4.K), dY, dY)
+    lib = _lib.load_lowbit()
+    work = _lb_work(lib.gpvae_dense_vjp_w4_workspace_bytes(dt, M, w4.K, w4.N), dev)
+    _lb_call("gpvae_dense_vjp_w4", dev, lib.gpvae_dense_vjp_w4, dt, M, w4.K, w4.N, _p(dY), dY.stride(0), _p(w4.codes),
+             _p(w4.exps), _p(None if act is None else act.codes), _p(dX), dX.stride(0), _p(work))
+    return dX
+
+
+def store_q8(X, relu=False, out=None):
+    """8-bit checkpoint of X [M, K] (float32, bfloat16 or float16), one power of two per 8 x 8 tile: a :class:`Q8`.
+    relu=True: (Y, Q8) with Y = max(X, 0), written to `out` if given (X itself: in place), and the checkpoint of Y.
+    A tile with an infinity or a NaN reads as NaN; its ReLU mask stays that of the values (NaN passes)."""
+    src = X
+    X = _lb_mat("store_q8", "X", X)
+    dt, dev = _lb_dt("store_q8", X), X.device
+    M, K = X.shape
+    if K < 1:
+        raise GpvaeError("store_q8: X must have at least one column; got %s" % (tuple(X.shape),))
+    if out is not None and not relu:
+        raise GpvaeError("store_q8: out is the ReLU's output (relu=True)")
+    if out is not None and X is not src and out is src:
+        raise GpvaeError("store_q8: in place needs unit column stride and rows that do not overlap")
+    Y = _lb_out("store_q8", out, (M, K), X, None) if relu else None
+    if Y is not None and M and Y.data_ptr() == X.data_ptr() and M > 1 and Y.stride(0) != X.stride(0):
+        raise GpvaeError("store_q8: in place needs equal strides")
+    mb, kp = (M + 7) // 8, (K + 31) // 32 * 32
+    codes = torch.empty((mb, kp, 8), dtype=torch.uint8, device=dev)
+    exps = torch.empty((mb, kp // 8), dtype=torch.uint8, device=dev)
+    _lb_call("gpvae_store_q8", dev, _lib.load_lowbit().gpvae_store_q8, dt, M, K, _p(X), X.stride(0), int(bool(relu)), _p(Y),
+             Y.stride(0) if relu else 0, _p(codes), _p(exps))
+    q8 = Q8(codes, exps, M, K, relu)
+    return (Y, q8) if relu else q8
+
+
+def load_q8(q8, dtype=torch.float32):
+    """The values [M, K] a checkpoint stands for (exact in float32 and bfloat16)."""
+    _dev(q8.codes)
+    out = torch.empty((q8.M, q8.K), dtype=dtype, device=q8.codes.device)
+    _lb_call("gpvae_load_q8", out.device, _lib.load_lowbit().gpvae_load_q8, _lb_dt("load_q8", out), q8.M, q8.K, int(q8.relu),
+             _p(q8.codes), _p(q8.exps), _p(out), q8.K)
+    return out
+
+
+def dense_grads_q8(q8, dY, out=None):
+    """(dW [K, N], db [N]) float32 of a dense layer y = x W + b from the 8-bit checkpoint of its input x [M, K] and
+    dY [M, N] (float32, bfloat16 or float16): dW = x~^T dY, db = sum of dY's rows.  out: optional pair (dW, db) of float32
+    tensors to write to (db may be None: not wanted)."""
+    dY = _lb_mat("dense_grads_q8", "dY", dY, rows=q8.M)
+    dt, dev, N = _lb_dt("dense_grads_q8", dY), dY.device, dY.shape[1]
+    if N < 1:
+        raise GpvaeError("dense_grads_q8: dY must have at least one column")
+    _lb_same("dense_grads_q8", dev, q8.codes)
+    if out is None:
+        dW = torch.empty((q8.K, N), dtype=torch.float32, device=dev)
+        db = torch.empty((N,), dtype=torch.float32, device=dev)
+    else:
+        dW, db = out
+        if (tuple(dW.shape) != (q8.K, N) or dW.dtype != torch.float32 or dW.device != dev or dW.stride(1) != 1
+                or dW.stride(0) < N):
+            raise GpvaeError("dense_grads_q8: dW must be float32 [%d, %d] on %s, unit column stride" % (q8.K, N, dev))
+        if db is not None and (tuple(db.shape) != (N,) or db.dtype != torch.float32 or db.device != dev or not db.is_contiguous()):
+            raise GpvaeError("dense_grads_q8: db must be contiguous float32 [%d] on %s" % (N, dev))
+    lib = _lib.load_lowbit()
+    work = _lb_work(lib.gpvae_dense_grads_q8_workspace_bytes(dt, q8.M, q8.K, N), dev)
+    _lb_call("gpvae_dense_grads_q8", dev, lib.gpvae_dense_grads_q8, dt, q8.M, q8.K, N, int(q8.relu), _p(q8.codes), _p(q8.exps),
+             _p(dY), dY.stride(0), _p(dW), dW.stride(0), _p(db), _p(work))
+    return dW, db

@@ -1,0 +1,370 @@
+"""GPU tests of the 4-bit dense layers and 8-bit checkpoints against the 64-bit NumPy oracle.
+
+Tolerance of a product: every piece product is exact in float32, so only the accumulation of at most 3 L + 8 terms and the
+last rounding to the output's type count: |err| <= (3 L + 8) 2^-23 sum|a b| + (eps / 2 + 2^-23) |y|, L the length of the sum,
+2^-23 twice the rounding of an addition (a matrix instruction may round a partial sum once more)."""
+import numpy as np
+import pytest
+import torch
+
+from gp_vae_amd import GpvaeError, ops
+from oracle import lowbit_oracle as orc
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+
+
+def np64(t):
+    return t.detach().to(torch.float64).cpu().numpy()
+
+
+def normal(rng, shape, dt, scale=1.0):
+    return torch.tensor(rng.standard_normal(shape) * scale, dtype=F32, device=DEV).to(dt)
+
+
+def close(got, want, absum, L, dt):
+    eps = torch.finfo(dt).eps
+    tiny = torch.finfo(dt).smallest_normal * eps  # below the smallest normal the step is fixed
+    tol = (3 * L + 8) * 2.0 ** -23 * absum + (eps / 2 + 2.0 ** -23) * np.abs(want) + tiny
+    err = np.abs(np64(got) - want)
+    bad = ~(err <= tol)
+    assert not bad.any(), "worst %g of its tolerance at %s" % (np.nanmax(err / tol), np.argwhere(bad)[:3].tolist())
+
+
+def w4_np(w4):
+    return orc.load_w4(w4.codes.cpu().numpy(), w4.exps.cpu().numpy(), w4.K, w4.N)
+
+
+def q8_np(q):
+    return orc.load_q8(q.codes.cpu().numpy(), q.exps.cpu().numpy(), q.M, q.K, q.relu)
+
+
+def strided(t, pad_rows=0, lead=3, shift=1):
+    """The same matrix inside a larger buffer: other leading dimension, unaligned base."""
+    M, K = t.shape
+    buf = torch.full((M + 1, K + lead + shift), 7.0, dtype=t.dtype, device=t.device)
+    v = buf[:M, shift:shift + K]
+    v.copy_(t)
+    return buf, v
+
+
+# ---- formats ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("K,N", [(1, 1), (8, 8), (32, 32), (50, 300), (33, 65), (7, 129), (100, 31)])
+def test_quant_w4_is_the_formats_definition(K, N, dt):
+    rng = np.random.default_rng(K * 1000 + N)
+    W = normal(rng, (K, N), dt) * torch.tensor(10.0 ** rng.integers(-3, 3, (K, 1)), dtype=dt, device=DEV)
+    _, V = strided(W)
+    for M in (W, V):
+        w4 = ops.quant_w4(M)
+        c, e = orc.quant_w4(np64(W))
+        assert np.array_equal(w4.codes.cpu().numpy().view(np.uint32), c) and np.array_equal(w4.exps.cpu().numpy(), e)
+    for out in (F32, BF16):
+        assert np.array_equal(np64(ops.load_w4(w4, out)), orc.load_w4(c, e, K, N))
+
+
+def test_quant_w4_special_values():
+    W = torch.zeros((40, 48), device=DEV)
+    W[0, 0], W[0, 9], W[0, 17], W[0, 25] = float("inf"), float("nan"), 3.4e38, 1e-45
+    W[8, :7] = torch.tensor([.25, .75, 1.25, 1.75, 2.5, 3.5, 5.0])   # ties, with the tile's 6 below
+    W[9, 0] = 6.0
+    W[16, :8] = torch.tensor([1e-38, -2e-38, 3e-39, -1e-45, 0.0, -0.0, 1.2e-38, 5e-39])
+    w4 = ops.quant_w4(W)
+    c, e = orc.quant_w4(np64(W))
+    assert np.array_equal(w4.codes.cpu().numpy().view(np.uint32), c) and np.array_equal(w4.exps.cpu().numpy(), e)
+    got = np64(ops.load_w4(w4))
+    assert np.isnan(got[:8, :16]).all() and np.isfinite(got[:8, 16:]).all() and np.isfinite(got[8:]).all()
+    assert np.array_equal(got, orc.load_w4(c, e, 40, 48), equal_nan=True)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,K", [(1, 1), (8, 8), (8, 32), (100, 35), (13, 129), (257, 64), (3, 1000)])
+@pytest.mark.parametrize("relu", [False, True])
+def test_store_q8_is_the_formats_definition(M, K, relu, dt):
+    rng = np.random.default_rng(M * 1000 + K)
+    X = normal(rng, (M, K), dt) * torch.tensor(10.0 ** rng.integers(-3, 3, (1, K)), dtype=dt, device=DEV)
+    Yw, c, e = orc.store_q8(np64(X), relu)
+    buf, V = strided(X)
+    for src in (X, V):
+        if relu:
+            Y, q = ops.store_q8(src, relu=True)
+            assert np.array_equal(np64(Y), Yw)
+        else:
+            q = ops.store_q8(src)
+        assert np.array_equal(q.codes.cpu().numpy(), c) and np.array_equal(q.exps.cpu().numpy(), e)
+    assert np.array_equal(np64(ops.load_q8(q)), orc.load_q8(c, e, M, K, relu))
+    assert np.array_equal(np64(ops.load_q8(q, BF16)), orc.load_q8(c, e, M, K, relu))
+    if relu:  # in place, inside a larger buffer whose rest stays as it was
+        Y, q = ops.store_q8(V, relu=True, out=V)
+        assert Y is V and np.array_equal(np64(V), Yw) and np.array_equal(q.codes.cpu().numpy(), c)
+        rest = buf.clone()
+        rest[:M, 1:1 + K] = 7.0
+        assert (rest == 7.0).all()
+
+
+@pytest.mark.parametrize("relu", [False, True])
+def test_store_q8_special_values(relu):
+    X = torch.zeros((16, 64), device=DEV)
+    X[0, 0], X[1, 1], X[0, 2], X[2, 9], X[0, 17], X[0, 25] = float("inf"), -1.0, 2.0, float("nan"), 3.4e38, 1e-45
+    X[3, 10], X[4, 33] = -float("inf"), -float("inf")
+    X[8, :8] = torch.tensor([1.0, 1e-6, -1e-6, 254.5 / 255, .5 / 255, 1.5 / 255, 2.5 / 255, 1e-45])
+    Yw, c, e = orc.store_q8(np64(X), relu)
+    q = ops.store_q8(X, relu=relu)
+    if relu:
+        Y, q = q
+        assert np.array_equal(np64(Y), Yw, equal_nan=True)
+        mask = q.codes.cpu().numpy().transpose(0, 2, 1).reshape(16, 64) != 0
+        assert np.array_equal(mask, ~(np64(X) <= 0))
+    assert np.array_equal(q.codes.cpu().numpy(), c) and np.array_equal(q.exps.cpu().numpy(), e)
+    assert np.array_equal(np64(ops.load_q8(q)), orc.load_q8(c, e, 16, 64, relu), equal_nan=True)
+
+
+# ---- products ---------------------------------------------------------------------------------------------------------
+SHAPES = [(1, 50, 4096), (1, 1, 1), (2, 35, 300), (3, 300, 17), (16, 64, 128), (17, 1024, 65), (33, 31, 1000), (64, 100, 96),
+          (65, 700, 33), (100, 33, 625), (130, 257, 260), (256, 96, 129), (300, 513, 1030)]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_dense_w4(M, K, N, dt):
+    rng = np.random.default_rng(M + 10 * K + 100 * N)
+    w4 = ops.quant_w4(normal(rng, (K, N), F32, K ** -0.5))
+    X, b = normal(rng, (M, K), dt), normal(rng, (N,), dt)
+    Wd, Xd, bd = w4_np(w4), np64(X), np64(b)
+    S = np.abs(Xd) @ np.abs(Wd) + np.abs(bd)
+    close(ops.dense_w4(X, w4), Xd @ Wd, S, K, dt)
+    Y = ops.dense_w4(X, w4, b, relu=True)
+    close(Y, orc.dense(Xd, Wd, bd, True), S, K, dt)
+    assert torch.equal(Y, ops.dense_w4(X, w4, b, relu=True))  # same inputs, same bits
+    buf, Xs = strided(X)
+    obuf = torch.full((M + 2, N + 5), 7.0, dtype=dt, device=DEV)
+    out = obuf[1:1 + M, 3:3 + N]
+    assert ops.dense_w4(Xs, w4, b, relu=True, out=out) is out and torch.equal(out, Y)
+    obuf[1:1 + M, 3:3 + N] = 7.0
+    assert (obuf == 7.0).all()                                # nothing beside the output was written
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_dense_vjp_w4(M, K, N, dt):
+    rng = np.random.default_rng(1 + M + 10 * K + 100 * N)
+    w4 = ops.quant_w4(normal(rng, (K, N), F32, K ** -0.5))
+    dY, A = normal(rng, (M, N), dt), normal(rng, (M, K), dt)
+    _, q = ops.store_q8(A, relu=True)
+    Wd, dYd = w4_np(w4), np64(dY)
+    S = np.abs(dYd) @ np.abs(Wd).T
+    close(ops.dense_vjp_w4(dY, w4), dYd @ Wd.T, S, N, dt)
+    dX = ops.dense_vjp_w4(dY, w4, q)
+    close(dX, orc.dense_vjp(dYd, Wd, np64(A) > 0), S, N, dt)
+    assert (dX[A <= 0] == 0).all() and torch.equal(dX, ops.dense_vjp_w4(dY, w4, q))
+    _, dYs = strided(dY)
+    obuf = torch.full((M + 2, K + 5), 7.0, dtype=dt, device=DEV)
+    out = obuf[1:1 + M, 3:3 + K]
+    assert ops.dense_vjp_w4(dYs, w4, q, out=out) is out and torch.equal(out, dX)
+    obuf[1:1 + M, 3:3 + K] = 7.0
+    assert (obuf == 7.0).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("relu", [False, True])
+@pytest.mark.parametrize("M,K,N", SHAPES + [(0, 5, 7), (1000, 50, 64), (2049, 33, 40)])
+def test_dense_grads_q8(M, K, N, relu, dt):
+    rng = np.random.default_rng(2 + M + 10 * K + 100 * N)
+    A, dY = normal(rng, (M, K), dt), normal(rng, (M, N), dt)
+    q = ops.store_q8(A, relu=relu)
+    q = q[1] if relu else q
+    Xd, dYd = q8_np(q), np64(dY)
+    dW, db = ops.dense_grads_q8(q, dY)
+    assert dW.dtype == F32 and db.dtype == F32
+    want = orc.dense_grads(Xd, dYd)
+    close(dW, want[0], np.abs(Xd).T @ np.abs(dYd), M, F32)
+    close(db, want[1], np.abs(dYd).sum(0), M, F32)
+    again = ops.dense_grads_q8(q, dY)
+    assert torch.equal(again[0], dW) and torch.equal(again[1], db)
+    if M:
+        _, dYs = strided(dY)
+        obuf = torch.full((K + 2, N + 5), 7.0, device=DEV)
+        out = obuf[1:1 + K, 3:3 + N]
+        ops.dense_grads_q8(q, dYs, out=(out, None))
+        assert torch.equal(out, dW)
+        obuf[1:1 + K, 3:3 + N] = 7.0
+        assert (obuf == 7.0).all()
+
+
+def test_gradients_agree_with_differences():
+    """d/dX and d/db of sum(C * dense) by central differences in 64 bits of the oracle's layer at the stored weights."""
+    rng = np.random.default_rng(9)
+    M, K, N = 5, 41, 37
+    w4 = ops.quant_w4(normal(rng, (K, N), F32))
+    X, Cc = normal(rng, (M, K), F32), normal(rng, (M, N), F32)
+    Wd, Xd, Cd = w4_np(w4), np64(X), np64(Cc)
+    f = lambda x: float((orc.dense(x, Wd, relu=True) * Cd).sum())
+    Y = ops.dense_w4(X, w4, relu=True)
+    dX = np64(ops.dense_vjp_w4(Cc * (Y > 0), w4))
+    for m, k in [(0, 0), (2, 17), (4, 40)]:
+        h = 1e-6
+        P, Q = Xd.copy(), Xd.copy()
+        P[m, k] += h
+        Q[m, k] -= h
+        assert abs((f(P) - f(Q)) / (2 * h) - dX[m, k]) < 1e-4 * np.abs(dX).max()
+
+
+@pytest.mark.parametrize("M", [1, 20, 200])
+def test_infinities_and_nan_reach_what_they_touch_and_nothing_else(M):
+    rng = np.random.default_rng(4)
+    K, N = 70, 90
+    W = normal(rng, (K, N), F32)
+    w4 = ops.quant_w4(W)
+    Wd = w4_np(w4)
+    X = normal(rng, (M, K), F32)
+    X[0, 3] = float("inf")
+    if M > 1:
+        X[1, 69] = float("nan")
+        X[M - 1, 0] = 3.4e38
+    Y, want = np64(ops.dense_w4(X, w4)), np64(X) @ Wd
+    with np.errstate(invalid="ignore", over="ignore"):
+        want32 = want.astype(np.float32).astype(np.float64)
+    rows = [r for r in range(M) if r not in (0, 1, M - 1)]
+    assert np.isfinite(Y[rows]).all()
+    nz = Wd[3] != 0
+    assert np.isnan(Y[0, ~nz]).all() and np.array_equal(Y[0, nz], np.sign(Wd[3, nz]) * np.inf)  # inf * 0 = NaN
+    if M > 1:
+        assert np.isnan(Y[1]).all()
+        big = np.abs(want32[M - 1]) < 3e38
+        assert np.isfinite(Y[M - 1][big]).all()
+    dY = normal(rng, (M, N), F32)
+    dY[0, 89] = -float("inf")
+    dX = np64(ops.dense_vjp_w4(dY, w4))
+    nz = Wd[:, 89] != 0
+    assert np.isfinite(dX[1:]).all() and np.array_equal(dX[0, nz], -np.sign(Wd[nz, 89]) * np.inf) and np.isnan(dX[0, ~nz]).all()
+    # a weight tile that is not finite: its rows' and columns' outputs are NaN, the others are not
+    W[9, 17] = float("nan")
+    bad = ops.quant_w4(W)
+    Y = ops.dense_w4(torch.ones((M, K), device=DEV), bad)
+    assert torch.isnan(Y[:, 16:24]).all() and torch.isfinite(Y[:, :16]).all() and torch.isfinite(Y[:, 24:]).all()
+    dX = ops.dense_vjp_w4(torch.ones((M, N), device=DEV), bad)
+    assert torch.isnan(dX[:, 8:16]).all() and torch.isfinite(dX[:, :8]).all() and torch.isfinite(dX[:, 16:]).all()
+    # the gradient of a checkpoint with a NaN in it
+    A = normal(rng, (M, K), F32)
+    A[0, 5] = float("nan")
+    dW, db = ops.dense_grads_q8(ops.store_q8(A), torch.ones((M, N), device=DEV))
+    assert torch.isnan(dW[:8]).all() and torch.isfinite(dW[8:]).all() and torch.isfinite(db).all()
+
+
+def test_float16_and_float32_extremes_keep_their_accuracy():
+    """Smallest and largest magnitudes of the types: every piece of the split carries its share."""
+    rng = np.random.default_rng(8)
+    w4 = ops.quant_w4(normal(rng, (64, 40), F32))
+    Wd = w4_np(w4)
+    for dt, lo, hi in ((F16, -24, 14), (F32, -100, 100), (BF16, -100, 100)):
+        X = (normal(rng, (6, 64), F32) * torch.tensor(2.0 ** rng.integers(lo, hi, (6, 1)), dtype=F32, device=DEV)).to(dt)
+        Xd = np64(X)
+        want = Xd @ Wd
+        top = torch.finfo(dt).max
+        ok = np.abs(want) < 0.9 * top
+        got, S = ops.dense_w4(X, w4), np.abs(Xd) @ np.abs(Wd)
+        close(torch.where(torch.tensor(ok, device=DEV), got, torch.zeros_like(got)), np.where(ok, want, 0), S, 64, dt)
+
+
+def test_other_layouts_and_empty_calls():
+    rng = np.random.default_rng(6)
+    K, N, M = 40, 50, 12
+    w4 = ops.quant_w4(normal(rng, (K, N), F32))
+    X = normal(rng, (M, K), F32)
+    assert torch.equal(ops.dense_w4(X.t().contiguous().t(), w4), ops.dense_w4(X, w4))            # column-major rows
+    one = normal(rng, (1, K), F32)
+    assert torch.equal(ops.dense_w4(one.expand(M, K), w4), ops.dense_w4(one.repeat(M, 1), w4))  # a broadcast row
+    g = torch.ones((), device=DEV).expand(M, N)
+    assert torch.equal(ops.dense_vjp_w4(g, w4), ops.dense_vjp_w4(g.contiguous(), w4))
+    q = ops.store_q8(X)
+    assert torch.equal(ops.dense_grads_q8(q, g)[0], ops.dense_grads_q8(q, g.contiguous())[0])
+    k1 = ops.quant_w4(normal(rng, (1, N), F32))
+    col = normal(rng, (M, 3), F32)[:, 1:2]
+    close(ops.dense_w4(col, k1), np64(col) @ w4_np(k1), np.abs(np64(col)) @ np.abs(w4_np(k1)), 1, F32)
+    assert ops.dense_w4(X[:0], w4).shape == (0, N) and ops.dense_vjp_w4(torch.empty((0, N), device=DEV), w4).shape == (0, K)
+    q0 = ops.store_q8(X[:0])
+    dW, db = ops.dense_grads_q8(q0, torch.empty((0, N), device=DEV))
+    assert ops.load_q8(q0).shape == (0, K) and (dW == 0).all() and (db == 0).all()
+
+
+def test_refusals():
+    w4 = ops.quant_w4(torch.ones((40, 50), device=DEV))
+    X = torch.ones((3, 40), device=DEV)
+    Y, q = ops.store_q8(X, relu=True)
+    bad = [lambda: ops.dense_w4(X.double(), w4), lambda: ops.dense_w4(X[:, :39], w4), lambda: ops.dense_w4(X[0], w4),
+           lambda: ops.dense_w4(X, w4, torch.ones(49, device=DEV)), lambda: ops.dense_w4(X, w4, torch.ones(50, device=DEV).half()),
+           lambda: ops.dense_w4(X, w4, out=torch.empty((3, 49), device=DEV)), lambda: ops.dense_w4(X, w4, out=torch.empty((50, 3), device=DEV).t()),
+           lambda: ops.dense_w4(X, w4, torch.ones(50)), lambda: ops.dense_vjp_w4(X, w4),
+           lambda: ops.dense_vjp_w4(torch.ones((3, 50), device=DEV), w4, ops.store_q8(X)),
+           lambda: ops.dense_vjp_w4(torch.ones((4, 50), device=DEV), w4, q), lambda: ops.quant_w4(torch.ones((0, 3), device=DEV)),
+           lambda: ops.store_q8(X, out=X), lambda: ops.store_q8(X.long()), lambda: ops.dense_grads_q8(q, torch.ones((4, 5), device=DEV)),
+           lambda: ops.dense_grads_q8(q, torch.ones((3, 0), device=DEV)),
+           lambda: ops.dense_grads_q8(q, X, out=(torch.empty((40, 39), device=DEV), None))]
+    sq = ops.quant_w4(torch.ones((40, 40), device=DEV))
+    bad.append(lambda: ops.dense_w4(X, sq, out=X))
+    for i, call in enumerate(bad):
+        with pytest.raises(GpvaeError):
+            call()
+            pytest.fail("call %d was not refused" % i)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^32 bytes of codes: rows and columns at both ends."""
+    K, N = 65600, 131104
+    g = torch.Generator(device=DEV)
+    g.manual_seed(1)
+    kb, np_ = K // 32, N
+    codes = torch.randint(-2 ** 31, 2 ** 31 - 1, (kb, np_, 4), dtype=torch.int32, device=DEV, generator=g)
+    exps = torch.randint(120, 125, (kb, np_ // 8, 4), dtype=torch.uint8, device=DEV, generator=g)
+    assert codes.numel() * 4 > 2 ** 32
+    w4 = ops.W4(codes, exps, K, N)
+    X = torch.randn((2, K), device=DEV, generator=g)
+    Y = ops.dense_w4(X, w4)
+    cut = ops.W4(codes[:, -64:].contiguous(), exps[:, -8:].contiguous(), K, 64)  # the last 64 columns
+    Wd = w4_np(cut)
+    close(Y[:, -64:], np64(X) @ Wd, np.abs(np64(X)) @ np.abs(Wd), K, F32)
+    dY = torch.randn((2, N), device=DEV, generator=g)
+    dX = ops.dense_vjp_w4(dY, w4)
+    cut = ops.W4(codes[-2:].contiguous(), exps[-2:].contiguous(), 64, N)         # the last 64 rows
+    Wd = w4_np(cut)
+    close(dX[:, -64:], np64(dY) @ Wd.T, np.abs(np64(dY)) @ np.abs(Wd).T, N, F32)
+
+
+# ---- streams and graphs -------------------------------------------------------------------------------------------------
+def test_side_stream_and_replayed_graph():
+    rng = np.random.default_rng(12)
+    M, K, N = 24, 96, 200
+    w4 = ops.quant_w4(normal(rng, (K, N), F32))
+    Xs = [normal(rng, (M, K), F32) for _ in range(4)]
+    dYs = [normal(rng, (M, N), F32) for _ in range(4)]
+    b = normal(rng, (N,), F32)
+
+    def step(X, dY):
+        A, q = ops.store_q8(X, relu=True)
+        Y = ops.dense_w4(A, w4, b, relu=True)
+        return (Y, ops.dense_vjp_w4(dY, w4, q), *ops.dense_grads_q8(q, dY))
+
+    want = [[t.clone() for t in step(X, dY)] for X, dY in zip(Xs, dYs)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step(Xs[0], dYs[0])
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, c) for a, c in zip(got, want[0]))
+    sx, sdy = Xs[0].clone(), dYs[0].clone()
+    graphs = []
+    for _ in range(2):  # two graphs of the same calls
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = step(sx, sdy)
+        graphs.append((g, outs))
+    for i in (1, 2, 3, 1, 0):
+        sx.copy_(Xs[i])
+        sdy.copy_(dYs[i])
+        for g, outs in graphs:
+            g.replay()
+            step(Xs[(i + 1) % 4], dYs[(i + 1) % 4])  # the program's own eager work between replays
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(outs, want[i])), i
