@@ -1,0 +1,128 @@
+// frag.hpp — fragments for v_mfma_f32_16x16x32_bf16 from the low-bit formats, and the exact split of floating operands.
+//
+// The instruction: lane l supplies A[l % 16][8 (l / 16) + i] and B[8 (l / 16) + i][l % 16], i = 0..7, and holds
+// D[4 (l / 16) + r][l % 16], r = 0..3.  Which reduction indices the four lane groups take is free as long as A and B agree.
+#pragma once
+#include "lowbit.hpp"
+
+namespace gpvae_lb {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+// ---- w4 -----------------------------------------------------------------------------------------------------------------
+// 8 codes -> 8 bfloat16 values; byte J of the tile-exponent word e is their exponent
+template <int J> __device__ __forceinline__ float w4_scale(uint32_t e) {
+  return __builtin_bit_cast(float, (J == 0 ? e << 23 : J == 1 ? e << 15 : J == 2 ? e << 7 : e >> 1) & 0x7f800000u);
+}
+__device__ __forceinline__ uint4 w4_frag(uint32_t w, float scale) {
+  return make_uint4(w4_pair<0>(w, scale), w4_pair<1>(w, scale), w4_pair<2>(w, scale), w4_pair<3>(w, scale));
+}
+
+// 8 x 8 transpose of nibbles inside groups of 8 lanes: the lane labelled a holds in[i] = T(i, a) and gets out[b] = T(a, b).
+// Labels are dealt so that the three exchange partners (label bit 0, 1, 2 flipped) are one DPP move each:
+// lane i, bits i2 i1 i0, carries label (i2, i1 ^ i2, i0 ^ i2), and i -> 7 - i flips label bit 2 alone.
+__device__ __forceinline__ int tr8_label(int lane) {
+  const int i2 = (lane >> 2) & 1;
+  return (i2 << 2) | ((((lane >> 1) & 1) ^ i2) << 1) | ((lane & 1) ^ i2);
+}
+struct Tr8 {
+  uint32_t sel4, sel2, rot, own;
+  __device__ __forceinline__ void init(int lane) {
+    const int b = tr8_label(lane);
+    sel4 = (b & 4) ? 0x03020706u : 0x05040100u;
+    sel2 = (b & 2) ? 0x03070105u : 0x06020400u;
+    rot = (b & 1) ? 4u : 28u;
+    own = (b & 1) ? 0xf0f0f0f0u : 0x0f0f0f0fu;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+    uint32_t p = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xf, 0xf, true);  // row_half_mirror
+    x = __builtin_amdgcn_perm(p, x, sel4);
+    p = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true);            // quad_perm [2,3,0,1]
+    x = __builtin_amdgcn_perm(p, x, sel2);
+    p = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true);            // quad_perm [1,0,3,2]
+    p = __builtin_amdgcn_alignbit(p, p, rot);
+    return (own & x) | (~own & p);
+  }
+};
+
+// ---- the floating operand as its exact sum of bfloat16 pieces -----------------------------------------------------------
+// Truncation, not rounding: the top 16 bits of a finite float are a finite bfloat16 whatever its size, the remainder is
+// exact, and float32's 24 bits are 8 + 8 + 8.  An infinity or a NaN goes into piece 0 alone: the remainder is taken of
+// the value clamped to the finite range, so that inf * w stays inf (inf - inf would make it NaN).
+template <typename T> struct Split;
+__device__ __forceinline__ uint32_t pack_hi(float a, float b) {  // top halves of a (low) and b (high)
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+}
+__device__ __forceinline__ float trunc_bf(float a) {
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) & 0xffff0000u);
+}
+__device__ __forceinline__ float finite(float a) {
+  return __builtin_amdgcn_fmed3f(a, -3.402823466e+38f, 3.402823466e+38f);
+}
+template <> struct Split<float> {
+  static constexpr int P = 3;
+  // two values -> one dword of each piece
+  __device__ static __forceinline__ void two(float a, float b, uint32_t *out) {
+    out[0] = pack_hi(a, b);
+    a = finite(a), b = finite(b);
+    a -= trunc_bf(a), b -= trunc_bf(b);
+    out[1] = pack_hi(a, b);
+    a -= trunc_bf(a), b -= trunc_bf(b);
+    out[2] = pack_hi(a, b);
+  }
+};
+template <> struct Split<_Float16> {
+  static constexpr int P = 2;
+  __device__ static __forceinline__ void two(_Float16 ha, _Float16 hb, uint32_t *out) {
+    float a = (float)ha, b = (float)hb;
+    out[0] = pack_hi(a, b);
+    a = finite(a), b = finite(b);
+    out[1] = pack_hi(a - trunc_bf(a), b - trunc_bf(b));
+  }
+};
+template <> struct Split<__bf16> {
+  static constexpr int P = 1;
+  __device__ static __forceinline__ void two(__bf16 a, __bf16 b, uint32_t *out) {
+    out[0] = (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
+  }
+};
+template <typename T> struct alignas(4 * sizeof(T)) Vec4 { T v[4]; };
+
+// v[0..3] = row[k .. k + 3], zero from L on; vec: the row is 4-element aligned
+template <typename T>
+__device__ __forceinline__ Vec4<T> load4(const T *row, int64_t k, int64_t L, bool vec) {
+  Vec4<T> v;
+  if (vec && k + 4 <= L) {
+    v = *reinterpret_cast<const Vec4<T> *>(row + k);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.v[i] = k + i < L ? row[k + i] : T(0.0f);
+  }
+  return v;
+}
+
+// the end of a dense layer's output element: bias, ReLU (NaN stays), or the checkpoint's mask; rounded once
+template <typename T, bool VJP> struct Epilogue {
+  const T *bias;
+  int relu;
+  const uint8_t *act;
+  int64_t act_kp;
+  T *out;
+  int64_t ldo;
+  __device__ __forceinline__ void operator()(int64_t m, int64_t o, float v) const {
+    if (VJP) {
+      if (act && act[((m >> 3) * act_kp + o) * 8 + (m & 7)] == 0) v = 0.0f;
+    } else {
+      if (bias) v += to_f32(bias[o]);
+      if (relu) v = v < 0.0f ? 0.0f : v;
+    }
+    out[m * ldo + o] = from_f32<T>(v);
+  }
+};
+
+}  // namespace gpvae_lb

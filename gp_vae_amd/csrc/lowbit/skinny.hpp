@@ -1,0 +1,217 @@
+// skinny.hpp — the product with 4-bit weights (VJP = false: Y = X W, reduction over K) and with their transpose
+// (VJP = true: dX = dY W^T, reduction over N) for few rows.
+//
+// What it has to do is read the codes once: K N / 2 bytes.  So each wave owns 32 outputs, streams codes straight
+// from memory into registers (2 KB per step of 128 reduction indices, the next step's loads in flight while this one
+// is multiplied) and multiplies them on the matrix pipe, whose 16 A rows carry the floating rows AND their pieces:
+// row p M + m of the operand image is piece p of row m, so one row of float32 costs one matrix instruction, not three.
+// The image sits in LDS; the waves of a workgroup share it, and split the reduction (WK) as far as there are
+// too few outputs to fill the chip; S workgroups split it further.  Pieces, waves and splits are added in a fixed order.
+#pragma once
+#include "frag.hpp"
+
+namespace gpvae_lb {
+
+constexpr int SK_WAVES = 8, SK_MAXROWS = 64;
+
+struct SkinnyPlan {
+  int rt;        // tiles of 16 operand rows
+  int wk;        // waves of a workgroup along the reduction (the others: along the outputs)
+  int chunk;     // reduction indices staged at a time (a multiple of 128 wk)
+  int splits;    // workgroups along the reduction
+  int steps;     // steps of 128 reduction indices of one split (a multiple of chunk / 128 unless it is the only chunk)
+  int64_t gx;    // workgroups along the outputs
+};
+static constexpr int skinny_lds(int rt) { return rt <= 1 ? 40 << 10 : rt == 2 ? 56 << 10 : 72 << 10; }
+
+static inline SkinnyPlan skinny_plan(int64_t rows, int64_t L, int64_t O) {
+  SkinnyPlan p;
+  p.rt = (int)cdiv(rows, 16);
+  const int64_t steps = cdiv(L, 128), tiles = cdiv(O, 32);
+  const int room = (int)((skinny_lds(p.rt) / rows - 16) / 256);  // steps whose image fits
+  p.wk = 1;
+  while (p.wk < SK_WAVES && 2 * p.wk <= steps && 2 * p.wk <= room && tiles * p.wk < 2048) p.wk *= 2;
+  const int64_t waves = tiles * p.wk;
+  int64_t s = 1;
+  if (waves < 1024) s = cdiv(2048, waves);
+  const int64_t most = steps / (4 * p.wk);  // a split keeps four steps for each of its waves
+  if (s > most) s = most;
+  if (s < 1) s = 1;
+  if (s > 64) s = 64;
+  int64_t per = cdiv(steps, s);
+  per = round_up(per, p.wk);
+  p.splits = (int)cdiv(steps, per);
+  p.steps = (int)per;
+  int64_t ch = room / p.wk * p.wk;
+  if (ch > per) ch = per;
+  p.chunk = (int)(ch * 128);
+  p.gx = cdiv(tiles, SK_WAVES / p.wk);
+  return p;
+}
+
+template <typename T, bool VJP, int RT>
+__global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_t L, int64_t O, const T *__restrict__ X,
+                                                               int64_t ldx, int vec, const uint4 *__restrict__ codes,
+                                                               const uint32_t *__restrict__ exps, int64_t Np, int64_t kbs,
+                                                               int wk_n, int steps, int chunk, float *__restrict__ part,
+                                                               Epilogue<T, VJP> ep) {
+  constexpr int P = Split<T>::P;
+  __shared__ __align__(16) unsigned char lds[skinny_lds(RT)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wk = wave & (wk_n - 1), wn = wave / wk_n;
+  const int c = lane >> 4, l16 = lane & 15;
+  const int64_t tile = (int64_t)blockIdx.x * (SK_WAVES / wk_n) + wn;  // 32 outputs
+  const bool live = tile * 32 < O;
+  const int rows = P * (int)M;
+  const int stride = chunk * 2 + 16;  // bytes of an image row: 16 more spread the rows over the banks
+  const int64_t s_all = cdiv(L, 128), s_lo = (int64_t)blockIdx.y * steps;
+  const int64_t s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
+  Tr8 tr;
+  if (VJP) tr.init(lane);
+  const int lab = tr8_label(lane), half = l16 >> 3;
+
+  uint4 cw[2];       // codes of one step: 16 bytes for each of two columns, or 8 bytes for each of four
+  uint32_t ce[VJP ? 4 : 2];
+  auto fetch = [&](int64_t s) {
+    if (!VJP) {
+      const int64_t kb = 4 * s + c;
+      const bool in = live && s < s_hi && kb < kbs;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int64_t n = tile * 32 + t * 16 + l16;
+        cw[t] = in ? codes[kb * Np + n] : make_uint4(0, 0, 0, 0);
+        ce[t] = in ? exps[kb * (Np / 8) + n / 8] : 0u;
+      }
+    } else {
+      uint2 *c2 = reinterpret_cast<uint2 *>(cw);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int64_t n0 = s * 128 + t * 32;
+        const bool in = live && s < s_hi && n0 < Np;
+        c2[t] = in ? reinterpret_cast<const uint2 *>(codes)[(tile * Np + n0 + c * 8 + lab) * 2 + half] : make_uint2(0, 0);
+        ce[t] = in ? exps[tile * (Np / 8) + n0 / 8 + c] : 0u;
+      }
+    }
+  };
+
+  f32x4_t acc[RT][2];
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) acc[r][t] = f32x4_t{0, 0, 0, 0};
+
+  fetch(s_lo + wk);
+  int a_off[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = r * 16 + l16;
+    a_off[r] = (row < rows ? row : rows - 1) * stride + (VJP ? c * 16 : c * 64);  // rows past the last: results unused
+  }
+  const int chunk_steps = chunk / 128;
+  for (int64_t s0 = s_lo; s0 < s_hi; s0 += chunk_steps) {
+    if (s0 != s_lo) __syncthreads();
+    {  // the image of reduction indices [128 s0, 128 s0 + chunk): 4 at a time, zeros past L
+      const int q = chunk / 4;
+      for (int i = tid; i < (int)M * q; i += 64 * SK_WAVES) {
+        const int m = i / q, k4 = i - m * q;
+        const Vec4<T> v = load4(X + m * ldx, s0 * 128 + k4 * 4, L, vec);
+        uint32_t a[P], b[P];
+        Split<T>::two(v.v[0], v.v[1], a);
+        Split<T>::two(v.v[2], v.v[3], b);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          *reinterpret_cast<uint2 *>(lds + (p * (int)M + m) * stride + k4 * 8) = make_uint2(a[p], b[p]);
+      }
+    }
+    __syncthreads();
+    for (int i = wk; i < chunk_steps; i += wk_n) {
+      const int64_t s = s0 + i;
+      if (s >= s_hi) break;
+      const uint4 w0 = cw[0], w1 = cw[1];
+      uint32_t e[VJP ? 4 : 2];
+#pragma unroll
+      for (int t = 0; t < (VJP ? 4 : 2); ++t) e[t] = ce[t];
+      fetch(s + wk_n);
+      const unsigned char *img = lds + i * 256;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint4 f0, f1;
+        if (!VJP) {
+          const uint32_t d0 = j == 0 ? w0.x : j == 1 ? w0.y : j == 2 ? w0.z : w0.w;
+          const uint32_t d1 = j == 0 ? w1.x : j == 1 ? w1.y : j == 2 ? w1.z : w1.w;
+          f0 = w4_frag(d0, j == 0 ? w4_scale<0>(e[0]) : j == 1 ? w4_scale<1>(e[0]) : j == 2 ? w4_scale<2>(e[0]) : w4_scale<3>(e[0]));
+          f1 = w4_frag(d1, j == 0 ? w4_scale<0>(e[1]) : j == 1 ? w4_scale<1>(e[1]) : j == 2 ? w4_scale<2>(e[1]) : w4_scale<3>(e[1]));
+        } else {  // columns: row tiles 2 half and 2 half + 1 of the block of 32
+          const uint32_t d0 = j == 0 ? w0.x : j == 1 ? w0.z : j == 2 ? w1.x : w1.z;
+          const uint32_t d1 = j == 0 ? w0.y : j == 1 ? w0.w : j == 2 ? w1.y : w1.w;
+          const uint32_t ej = e[VJP ? j : 0] >> (16 * half);
+          f0 = w4_frag(tr(d0), w4_scale<0>(ej));
+          f1 = w4_frag(tr(d1), w4_scale<1>(ej));
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const uint4 a = *reinterpret_cast<const uint4 *>(img + a_off[r] + (VJP ? j * 64 : j * 16));
+          acc[r][0] = mfma(a, f0, acc[r][0]);
+          acc[r][1] = mfma(a, f1, acc[r][1]);
+        }
+      }
+    }
+  }
+
+  // [wave][operand row][output of the wave's 32] -> sums over the waves of one output tile, then over the pieces
+  __syncthreads();
+  float *red = reinterpret_cast<float *>(lds);
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int row = r * 16 + 4 * c + v;
+        const int o = VJP ? (2 * half + t) * 8 + lab : t * 16 + l16;
+        if (row < rows) red[(wave * rows + row) * 32 + o] = acc[r][t][v];
+      }
+  __syncthreads();
+  const int outs = SK_WAVES / wk_n * 32;
+  for (int i = tid; i < (int)M * outs; i += 64 * SK_WAVES) {
+    const int m = i / outs, oo = i - m * outs, w = oo >> 5, col = oo & 31;
+    const int64_t o = ((int64_t)blockIdx.x * (SK_WAVES / wk_n) + w) * 32 + col;
+    if (o >= O) continue;
+    float v = 0.0f;
+#pragma unroll
+    for (int p = P - 1; p >= 0; --p)  // small pieces first
+      for (int k = 0; k < wk_n; ++k) v += red[((w * wk_n + k) * rows + p * (int)M + m) * 32 + col];
+    if (gridDim.y == 1) ep(m, o, v);
+    else part[((int64_t)blockIdx.y * M + m) * O + o] = v;
+  }
+}
+
+template <typename T, bool VJP>
+__global__ __launch_bounds__(256) void split_sum_kernel(int64_t M, int64_t O, int splits, const float *__restrict__ part,
+                                                        Epilogue<T, VJP> ep) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * O) return;
+  float v = 0.0f;
+  for (int s = 0; s < splits; ++s) v += part[s * M * O + i];
+  ep(i / O, i % O, v);
+}
+
+template <typename T, bool VJP>
+static void launch_skinny(hipStream_t st, const SkinnyPlan &p, int64_t M, int64_t L, int64_t O, const T *X, int64_t ldx,
+                          const void *codes, const void *exps, int64_t Np, int64_t kbs, float *part,
+                          const Epilogue<T, VJP> &ep) {
+  const int vec = reinterpret_cast<uintptr_t>(X) % (4 * sizeof(T)) == 0 && (ldx % 4 == 0 || M == 1);
+  const dim3 grid((unsigned)p.gx, (unsigned)p.splits);
+#define GO(RT)                                                                                                            \
+  hipLaunchKernelGGL((skinny_kernel<T, VJP, RT>), grid, dim3(64 * SK_WAVES), 0, st, M, L, O, X, ldx, vec,               \
+                     (const uint4 *)codes, (const uint32_t *)exps, Np, kbs, p.wk, p.steps, p.chunk, part, ep)
+  if (p.rt == 1) GO(1);
+  else if (p.rt == 2) GO(2);
+  else if (p.rt == 3) GO(3);
+  else GO(4);
+#undef GO
+  if (p.splits > 1)
+    hipLaunchKernelGGL((split_sum_kernel<T, VJP>), dim3((unsigned)cdiv(M * O, 256)), dim3(256), 0, st, M, O, p.splits, part, ep);
+}
+
+}  // namespace gpvae_lb

@@ -1,5 +1,5 @@
 // w4.hip — dense layers with weights in 4 bits: quantiser, reader, the product and the transposed product.
-#include "lowbit.hpp"
+#include "skinny.hpp"
 
 namespace gpvae_lb {
 
@@ -124,8 +124,19 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
   return 0;
 }
 
-extern "C" int64_t gpvae_dense_w4_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
-extern "C" int64_t gpvae_dense_vjp_w4_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
+// pieces of a floating operand of this type
+static inline int pieces(int dtype) { return dtype == GPVAE_LB_F32 ? 3 : dtype == GPVAE_LB_F16 ? 2 : 1; }
+static int64_t w4_workspace(int dtype, int64_t M, int64_t L, int64_t O) {
+  if (!dtype_ok(dtype) || M < 1 || L < 1 || O < 1 || pieces(dtype) * M > SK_MAXROWS) return 0;
+  const SkinnyPlan p = skinny_plan(pieces(dtype) * M, L, O);
+  return p.splits > 1 ? p.splits * M * O * 4 : 0;
+}
+extern "C" int64_t gpvae_dense_w4_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
+  return w4_workspace(dtype, M, K, N);
+}
+extern "C" int64_t gpvae_dense_vjp_w4_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
+  return w4_workspace(dtype, M, N, K);
+}
 
 extern "C" int gpvae_dense_w4(void *stream, int dtype, int64_t M, int64_t K, int64_t N, const void *X, int64_t ldx,
                               const void *codes, const void *exps, const void *bias, int relu, void *Y, int64_t ldy,
@@ -141,6 +152,17 @@ extern "C" int gpvae_dense_w4(void *stream, int dtype, int64_t M, int64_t K, int
   LB_REQUIRE(exps && aligned16(exps), 9, "%s: exps must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(Y && Y != X, 12, "%s: Y is NULL or X", fn);
   LB_REQUIRE(ldy >= N, 13, "%s: ldy < N", fn);
+  LB_REQUIRE(!w4_workspace(dtype, M, K, N) || (work && aligned16(work)), 14, "%s: work must be a 16-byte aligned device pointer", fn);
+  if (pieces(dtype) * M <= SK_MAXROWS) {
+    const SkinnyPlan p = skinny_plan(pieces(dtype) * M, K, N);
+#define GO(T)                                                                                                       \
+  launch_skinny<T, false>((hipStream_t)stream, p, M, K, N, (const T *)X, ldx, codes, exps, w4_np(N), w4_kb(K),    \
+                          (float *)work, Epilogue<T, false>{(const T *)bias, relu, nullptr, 0, (T *)Y, ldy})
+    LB_BY_DTYPE(dtype, GO);
+#undef GO
+    LB_CHECK_LAUNCH(fn);
+    return 0;
+  }
   const dim3 grid((unsigned)cdiv(N, 256), (unsigned)(M < 65535 ? M : 65535));
 #define GO(T)                                                                                                              \
   hipLaunchKernelGGL(dense_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, M, K, N, (const T *)X, ldx,            \
@@ -166,6 +188,17 @@ extern "C" int gpvae_dense_vjp_w4(void *stream, int dtype, int64_t M, int64_t K,
   LB_REQUIRE(!act_codes || aligned16(act_codes), 10, "%s: act_codes must be 16-byte aligned", fn);
   LB_REQUIRE(dX && dX != dY, 11, "%s: dX is NULL or dY", fn);
   LB_REQUIRE(lddx >= K, 12, "%s: lddx < K", fn);
+  LB_REQUIRE(!w4_workspace(dtype, M, N, K) || (work && aligned16(work)), 13, "%s: work must be a 16-byte aligned device pointer", fn);
+  if (pieces(dtype) * M <= SK_MAXROWS) {
+    const SkinnyPlan p = skinny_plan(pieces(dtype) * M, N, K);
+#define GO(T)                                                                                                         \
+  launch_skinny<T, true>((hipStream_t)stream, p, M, N, K, (const T *)dY, lddy, codes, exps, w4_np(N), w4_kb(K),     \
+                         (float *)work, Epilogue<T, true>{nullptr, 0, (const uint8_t *)act_codes, q8_kp(K), (T *)dX, lddx})
+    LB_BY_DTYPE(dtype, GO);
+#undef GO
+    LB_CHECK_LAUNCH(fn);
+    return 0;
+  }
   const dim3 grid((unsigned)cdiv(K, 256), (unsigned)(M < 65535 ? M : 65535));
 #define GO(T)                                                                                                            \
   hipLaunchKernelGGL(dense_vjp_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, M, K, N, (const T *)dY, lddy,    \
