@@ -91,13 +91,13 @@ template <> struct Split<__bf16> {
     out[0] = (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
   }
 };
-template <typename T> struct alignas(4 * sizeof(T)) Vec4 { T v[4]; };
+// four elements at any element-aligned address: one vector load (unaligned access is on)
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Vec4 { T v[4]; };
 
-// v[0..3] = row[k .. k + 3], zero from L on; vec: the row is 4-element aligned
-template <typename T>
-__device__ __forceinline__ Vec4<T> load4(const T *row, int64_t k, int64_t L, bool vec) {
+// v[0..3] = row[k .. k + 3], zero from L on
+template <typename T> __device__ __forceinline__ Vec4<T> load4(const T *row, int64_t k, int64_t L) {
   Vec4<T> v;
-  if (vec && k + 4 <= L) {
+  if (k + 4 <= L) {
     v = *reinterpret_cast<const Vec4<T> *>(row + k);
   } else {
 #pragma unroll
@@ -124,5 +124,16 @@ template <typename T, bool VJP> struct Epilogue {
     out[m * ldo + o] = from_f32<T>(v);
   }
 };
+
+// the sum of the partial outputs [splits][M][O] in order, and the epilogue
+template <typename T, bool VJP>
+__global__ __launch_bounds__(256) void split_sum_kernel(int64_t M, int64_t O, int splits, const float *__restrict__ part,
+                                                        Epilogue<T, VJP> ep) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * O) return;
+  float v = 0.0f;
+  for (int s = 0; s < splits; ++s) v += part[s * M * O + i];
+  ep(i / O, i % O, v);
+}
 
 }  // namespace gpvae_lb

@@ -31,9 +31,8 @@ static inline SkinnyPlan skinny_plan(int64_t rows, int64_t L, int64_t O) {
   const int room = (int)((skinny_lds(p.rt) / rows - 16) / 256);  // steps whose image fits
   p.wk = 1;
   while (p.wk < SK_WAVES && 2 * p.wk <= steps && 2 * p.wk <= room && tiles * p.wk < 2048) p.wk *= 2;
-  const int64_t waves = tiles * p.wk;
-  int64_t s = 1;
-  if (waves < 1024) s = cdiv(2048, waves);
+  p.gx = cdiv(tiles, SK_WAVES / p.wk);
+  int64_t s = p.gx < 256 ? cdiv(512, p.gx) : 1;
   const int64_t most = steps / (4 * p.wk);  // a split keeps four steps for each of its waves
   if (s > most) s = most;
   if (s < 1) s = 1;
@@ -45,13 +44,12 @@ static inline SkinnyPlan skinny_plan(int64_t rows, int64_t L, int64_t O) {
   int64_t ch = room / p.wk * p.wk;
   if (ch > per) ch = per;
   p.chunk = (int)(ch * 128);
-  p.gx = cdiv(tiles, SK_WAVES / p.wk);
   return p;
 }
 
 template <typename T, bool VJP, int RT>
 __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_t L, int64_t O, const T *__restrict__ X,
-                                                               int64_t ldx, int vec, const uint4 *__restrict__ codes,
+                                                               int64_t ldx, const uint4 *__restrict__ codes,
                                                                const uint32_t *__restrict__ exps, int64_t Np, int64_t kbs,
                                                                int wk_n, int steps, int chunk, float *__restrict__ part,
                                                                Epilogue<T, VJP> ep) {
@@ -114,7 +112,7 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
       const int q = chunk / 4;
       for (int i = tid; i < (int)M * q; i += 64 * SK_WAVES) {
         const int m = i / q, k4 = i - m * q;
-        const Vec4<T> v = load4(X + m * ldx, s0 * 128 + k4 * 4, L, vec);
+        const Vec4<T> v = load4(X + m * ldx, s0 * 128 + k4 * 4, L);
         uint32_t a[P], b[P];
         Split<T>::two(v.v[0], v.v[1], a);
         Split<T>::two(v.v[2], v.v[3], b);
@@ -187,23 +185,12 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
 }
 
 template <typename T, bool VJP>
-__global__ __launch_bounds__(256) void split_sum_kernel(int64_t M, int64_t O, int splits, const float *__restrict__ part,
-                                                        Epilogue<T, VJP> ep) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * O) return;
-  float v = 0.0f;
-  for (int s = 0; s < splits; ++s) v += part[s * M * O + i];
-  ep(i / O, i % O, v);
-}
-
-template <typename T, bool VJP>
 static void launch_skinny(hipStream_t st, const SkinnyPlan &p, int64_t M, int64_t L, int64_t O, const T *X, int64_t ldx,
                           const void *codes, const void *exps, int64_t Np, int64_t kbs, float *part,
                           const Epilogue<T, VJP> &ep) {
-  const int vec = reinterpret_cast<uintptr_t>(X) % (4 * sizeof(T)) == 0 && (ldx % 4 == 0 || M == 1);
   const dim3 grid((unsigned)p.gx, (unsigned)p.splits);
 #define GO(RT)                                                                                                            \
-  hipLaunchKernelGGL((skinny_kernel<T, VJP, RT>), grid, dim3(64 * SK_WAVES), 0, st, M, L, O, X, ldx, vec,               \
+  hipLaunchKernelGGL((skinny_kernel<T, VJP, RT>), grid, dim3(64 * SK_WAVES), 0, st, M, L, O, X, ldx,                    \
                      (const uint4 *)codes, (const uint32_t *)exps, Np, kbs, p.wk, p.steps, p.chunk, part, ep)
   if (p.rt == 1) GO(1);
   else if (p.rt == 2) GO(2);

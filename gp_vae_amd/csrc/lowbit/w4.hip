@@ -1,5 +1,6 @@
 // w4.hip — dense layers with weights in 4 bits: quantiser, reader, the product and the transposed product.
 #include "skinny.hpp"
+#include "tile.hpp"
 
 namespace gpvae_lb {
 
@@ -44,36 +45,6 @@ __global__ __launch_bounds__(256) void load_w4_kernel(int64_t K, int64_t N, cons
   const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, Np = w4_np(N);
   if (n >= N) return;
   for (int64_t k = blockIdx.y; k < K; k += gridDim.y) out[k * ldo + n] = from_f32<T>(w4_value(codes, exps, Np, k, n));
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void dense_w4_kernel(int64_t M, int64_t K, int64_t N, const T *__restrict__ X, int64_t ldx,
-                                                       const uint32_t *__restrict__ codes, const uint8_t *__restrict__ exps,
-                                                       const T *__restrict__ bias, int relu, T *__restrict__ Y, int64_t ldy) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, Np = w4_np(N);
-  if (n >= N) return;
-  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
-    float a = 0.0f;
-    for (int64_t k = 0; k < K; ++k) a = fmaf(to_f32(X[m * ldx + k]), w4_value(codes, exps, Np, k, n), a);
-    if (bias) a += to_f32(bias[n]);
-    if (relu) a = a < 0.0f ? 0.0f : a;
-    Y[m * ldy + n] = from_f32<T>(a);
-  }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void dense_vjp_w4_kernel(int64_t M, int64_t K, int64_t N, const T *__restrict__ dY,
-                                                           int64_t lddy, const uint32_t *__restrict__ codes,
-                                                           const uint8_t *__restrict__ exps, const uint8_t *__restrict__ act,
-                                                           T *__restrict__ dX, int64_t lddx) {
-  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, Np = w4_np(N);
-  if (k >= K) return;
-  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
-    float a = 0.0f;
-    for (int64_t n = 0; n < N; ++n) a = fmaf(to_f32(dY[m * lddy + n]), w4_value(codes, exps, Np, k, n), a);
-    if (act && act[((m / 8) * q8_kp(K) + k) * 8 + m % 8] == 0) a = 0.0f;
-    dX[m * lddx + k] = from_f32<T>(a);
-  }
 }
 
 static int check_w4(const char *fn, int dtype, int64_t K, int64_t N, int kn_arg) {
@@ -127,9 +98,27 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
 // pieces of a floating operand of this type
 static inline int pieces(int dtype) { return dtype == GPVAE_LB_F32 ? 3 : dtype == GPVAE_LB_F16 ? 2 : 1; }
 static int64_t w4_workspace(int dtype, int64_t M, int64_t L, int64_t O) {
-  if (!dtype_ok(dtype) || M < 1 || L < 1 || O < 1 || pieces(dtype) * M > SK_MAXROWS) return 0;
-  const SkinnyPlan p = skinny_plan(pieces(dtype) * M, L, O);
-  return p.splits > 1 ? p.splits * M * O * 4 : 0;
+  if (!dtype_ok(dtype) || M < 1 || L < 1 || O < 1) return 0;
+  const int P = pieces(dtype);
+  if (P * M <= SK_MAXROWS) {
+    const SkinnyPlan p = skinny_plan(P * M, L, O);
+    return p.splits > 1 ? p.splits * M * O * 4 : 0;
+  }
+  const TilePlan p = tile_plan(P, M, L, O, false);
+  return p.plane_bytes + (p.splits > 1 ? p.splits * M * O * 4 : 0);
+}
+template <typename T, bool VJP>
+static void run_w4(hipStream_t st, int64_t M, int64_t L, int64_t O, const void *X, int64_t ldx, const void *codes,
+                   const void *exps, int64_t Np, int64_t kbs, void *work, const Epilogue<T, VJP> &ep) {
+  constexpr int P = Split<T>::P;
+  if (P * M <= SK_MAXROWS) {
+    launch_skinny<T, VJP>(st, skinny_plan(P * M, L, O), M, L, O, (const T *)X, ldx, codes, exps, Np, kbs, (float *)work, ep);
+  } else {
+    // a bfloat16 operand is its own plane where its rows can be read 16 bytes at a time to the end of the last step
+    const bool direct = P == 1 && L % 64 == 0 && ldx % 8 == 0 && aligned16(X);
+    launch_tile<T, VJP>(st, tile_plan(P, M, L, O, direct), M, L, O, (const T *)X, ldx, codes, exps, Np, kbs,
+                        (unsigned char *)work, ep);
+  }
 }
 extern "C" int64_t gpvae_dense_w4_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
   return w4_workspace(dtype, M, K, N);
@@ -153,20 +142,9 @@ extern "C" int gpvae_dense_w4(void *stream, int dtype, int64_t M, int64_t K, int
   LB_REQUIRE(Y && Y != X, 12, "%s: Y is NULL or X", fn);
   LB_REQUIRE(ldy >= N, 13, "%s: ldy < N", fn);
   LB_REQUIRE(!w4_workspace(dtype, M, K, N) || (work && aligned16(work)), 14, "%s: work must be a 16-byte aligned device pointer", fn);
-  if (pieces(dtype) * M <= SK_MAXROWS) {
-    const SkinnyPlan p = skinny_plan(pieces(dtype) * M, K, N);
-#define GO(T)                                                                                                       \
-  launch_skinny<T, false>((hipStream_t)stream, p, M, K, N, (const T *)X, ldx, codes, exps, w4_np(N), w4_kb(K),    \
-                          (float *)work, Epilogue<T, false>{(const T *)bias, relu, nullptr, 0, (T *)Y, ldy})
-    LB_BY_DTYPE(dtype, GO);
-#undef GO
-    LB_CHECK_LAUNCH(fn);
-    return 0;
-  }
-  const dim3 grid((unsigned)cdiv(N, 256), (unsigned)(M < 65535 ? M : 65535));
-#define GO(T)                                                                                                              \
-  hipLaunchKernelGGL(dense_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, M, K, N, (const T *)X, ldx,            \
-                     (const uint32_t *)codes, (const uint8_t *)exps, (const T *)bias, relu, (T *)Y, ldy)
+#define GO(T)                                                                                                        \
+  run_w4<T, false>((hipStream_t)stream, M, K, N, X, ldx, codes, exps, w4_np(N), w4_kb(K), work,                     \
+                   Epilogue<T, false>{(const T *)bias, relu, nullptr, 0, (T *)Y, ldy})
   LB_BY_DTYPE(dtype, GO);
 #undef GO
   LB_CHECK_LAUNCH(fn);
@@ -189,20 +167,9 @@ extern "C" int gpvae_dense_vjp_w4(void *stream, int dtype, int64_t M, int64_t K,
   LB_REQUIRE(dX && dX != dY, 11, "%s: dX is NULL or dY", fn);
   LB_REQUIRE(lddx >= K, 12, "%s: lddx < K", fn);
   LB_REQUIRE(!w4_workspace(dtype, M, N, K) || (work && aligned16(work)), 13, "%s: work must be a 16-byte aligned device pointer", fn);
-  if (pieces(dtype) * M <= SK_MAXROWS) {
-    const SkinnyPlan p = skinny_plan(pieces(dtype) * M, N, K);
-#define GO(T)                                                                                                         \
-  launch_skinny<T, true>((hipStream_t)stream, p, M, N, K, (const T *)dY, lddy, codes, exps, w4_np(N), w4_kb(K),     \
-                         (float *)work, Epilogue<T, true>{nullptr, 0, (const uint8_t *)act_codes, q8_kp(K), (T *)dX, lddx})
-    LB_BY_DTYPE(dtype, GO);
-#undef GO
-    LB_CHECK_LAUNCH(fn);
-    return 0;
-  }
-  const dim3 grid((unsigned)cdiv(K, 256), (unsigned)(M < 65535 ? M : 65535));
-#define GO(T)                                                                                                            \
-  hipLaunchKernelGGL(dense_vjp_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, M, K, N, (const T *)dY, lddy,    \
-                     (const uint32_t *)codes, (const uint8_t *)exps, (const uint8_t *)act_codes, (T *)dX, lddx)
+#define GO(T)                                                                                                        \
+  run_w4<T, true>((hipStream_t)stream, M, N, K, dY, lddy, codes, exps, w4_np(N), w4_kb(K), work,                    \
+                  Epilogue<T, true>{nullptr, 0, (const uint8_t *)act_codes, q8_kp(K), (T *)dX, lddx})
   LB_BY_DTYPE(dtype, GO);
 #undef GO
   LB_CHECK_LAUNCH(fn);
