@@ -10,7 +10,7 @@ namespace gpvae_lb {
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
-__device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
+__device__ __forceinline__ f32x4_t mfma(u32x4 a, u32x4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
@@ -19,8 +19,8 @@ __device__ __forceinline__ f32x4_t mfma(uint4 a, uint4 b, f32x4_t c) {
 template <int J> __device__ __forceinline__ float w4_scale(uint32_t e) {
   return __builtin_bit_cast(float, (J == 0 ? e << 23 : J == 1 ? e << 15 : J == 2 ? e << 7 : e >> 1) & 0x7f800000u);
 }
-__device__ __forceinline__ uint4 w4_frag(uint32_t w, float scale) {
-  return make_uint4(w4_pair<0>(w, scale), w4_pair<1>(w, scale), w4_pair<2>(w, scale), w4_pair<3>(w, scale));
+__device__ __forceinline__ u32x4 w4_frag(uint32_t w, float scale) {
+  return u32x4{w4_pair<0>(w, scale), w4_pair<1>(w, scale), w4_pair<2>(w, scale), w4_pair<3>(w, scale)};
 }
 
 // 8 x 8 transpose of nibbles inside groups of 8 lanes: the lane labelled a holds in[i] = T(i, a) and gets out[b] = T(a, b).
@@ -106,7 +106,8 @@ template <typename T> __device__ __forceinline__ Vec4<T> load4(const T *row, int
   return v;
 }
 
-// the end of a dense layer's output element: bias, ReLU (NaN stays), or the checkpoint's mask; rounded once
+// The end of a dense layer's output element: bias and ReLU (NaN stays), or the checkpoint's mask; rounded once.  What an
+// element needs from memory is loaded by the caller ahead of a batch of stores: a load behind a store waits for it.
 template <typename T, bool VJP> struct Epilogue {
   const T *bias;
   int relu;
@@ -114,11 +115,19 @@ template <typename T, bool VJP> struct Epilogue {
   int64_t act_kp;
   T *out;
   int64_t ldo;
-  __device__ __forceinline__ void operator()(int64_t m, int64_t o, float v) const {
+  __device__ __forceinline__ float bias_at(int64_t o) const { return !VJP && bias ? to_f32(bias[o]) : 0.0f; }
+  // mask byte of one element; the four bytes of rows m .. m + 3, m a multiple of 4
+  __device__ __forceinline__ uint32_t mask_at(int64_t m, int64_t o) const {
+    return VJP && act ? act[((m >> 3) * act_kp + o) * 8 + (m & 7)] : 1u;
+  }
+  __device__ __forceinline__ uint32_t mask4_at(int64_t m, int64_t o) const {
+    return VJP && act ? *reinterpret_cast<const uint32_t *>(act + ((m >> 3) * act_kp + o) * 8 + (m & 7)) : 0x01010101u;
+  }
+  __device__ __forceinline__ void store(int64_t m, int64_t o, float v, float b, uint32_t mask) const {
     if (VJP) {
-      if (act && act[((m >> 3) * act_kp + o) * 8 + (m & 7)] == 0) v = 0.0f;
+      if (!mask) v = 0.0f;
     } else {
-      if (bias) v += to_f32(bias[o]);
+      if (bias) v += b;
       if (relu) v = v < 0.0f ? 0.0f : v;
     }
     out[m * ldo + o] = from_f32<T>(v);
@@ -131,9 +140,12 @@ __global__ __launch_bounds__(256) void split_sum_kernel(int64_t M, int64_t O, in
                                                         Epilogue<T, VJP> ep) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= M * O) return;
+  const int64_t m = i / O, o = i - m * O;
+  const float b = ep.bias_at(o);
+  const uint32_t mask = ep.mask_at(m, o);
   float v = 0.0f;
   for (int s = 0; s < splits; ++s) v += part[s * M * O + i];
-  ep(i / O, i % O, v);
+  ep.store(m, o, v, b, mask);
 }
 
 }  // namespace gpvae_lb

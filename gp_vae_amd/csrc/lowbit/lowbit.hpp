@@ -40,6 +40,9 @@ static inline __host__ __device__ int64_t round_up(int64_t a, int64_t b) { retur
 static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static inline bool dtype_ok(int dt) { return dt == GPVAE_LB_F32 || dt == GPVAE_LB_BF16 || dt == GPVAE_LB_F16; }
 
+// (the compiler keeps arrays of these in registers; of HIP's uint4 / uint2 structures it does not)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 
 // ---- floating element types --------------------------------------------------------------------------------

@@ -1,5 +1,5 @@
 // q8.hip — activation checkpoints in 8 bits: writer (with the ReLU), reader, parameter gradients of a dense layer.
-#include "lowbit.hpp"
+#include "grads.hpp"
 
 namespace gpvae_lb {
 
@@ -51,25 +51,6 @@ __global__ __launch_bounds__(256) void load_q8_kernel(int64_t M, int64_t K, cons
   const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (k >= K) return;
   for (int64_t m = blockIdx.y; m < M; m += gridDim.y) out[m * ldo + k] = from_f32<T>(q8_value<RELU>(codes, exps, q8_kp(K), m, k));
-}
-
-template <typename T, bool RELU>
-__global__ __launch_bounds__(256) void dense_grads_q8_kernel(int64_t M, int64_t K, int64_t N, const uint8_t *__restrict__ codes,
-                                                             const uint8_t *__restrict__ exps, const T *__restrict__ dY,
-                                                             int64_t lddy, float *__restrict__ dW, int64_t lddw,
-                                                             float *__restrict__ db) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
-  for (int64_t k = blockIdx.y; k < K; k += gridDim.y) {
-    float a = 0.0f;
-    for (int64_t m = 0; m < M; ++m) a = fmaf(q8_value<RELU>(codes, exps, q8_kp(K), m, k), to_f32(dY[m * lddy + n]), a);
-    dW[k * lddw + n] = a;
-  }
-  if (db && blockIdx.y == 0) {
-    float a = 0.0f;
-    for (int64_t m = 0; m < M; ++m) a += to_f32(dY[m * lddy + n]);
-    db[n] = a;
-  }
 }
 
 static int check_q8(const char *fn, int dtype, int64_t M, int64_t K) {
@@ -129,7 +110,11 @@ extern "C" int gpvae_load_q8(void *stream, int dtype, int64_t M, int64_t K, int 
   return 0;
 }
 
-extern "C" int64_t gpvae_dense_grads_q8_workspace_bytes(int, int64_t, int64_t, int64_t) { return 0; }
+extern "C" int64_t gpvae_dense_grads_q8_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
+  if (!dtype_ok(dtype) || M < 0 || K < 1 || N < 1) return 0;
+  const GradsPlan p = grads_plan(M, K, N);
+  return p.splits > 1 ? p.splits * (K + 1) * N * 4 : 0;
+}
 
 extern "C" int gpvae_dense_grads_q8(void *stream, int dtype, int64_t M, int64_t K, int64_t N, int relu, const void *codes,
                                     const void *exps, const void *dY, int64_t lddy, float *dW, int64_t lddw, float *db,
@@ -143,10 +128,11 @@ extern "C" int gpvae_dense_grads_q8(void *stream, int dtype, int64_t M, int64_t 
   LB_REQUIRE(M == 0 || lddy >= N, 10, "%s: lddy < N", fn);
   LB_REQUIRE(dW, 11, "%s: dW is NULL", fn);
   LB_REQUIRE(lddw >= N, 12, "%s: lddw < N", fn);
-  const dim3 grid((unsigned)cdiv(N, 256), (unsigned)(K < 65535 ? K : 65535));
+  LB_REQUIRE(!gpvae_dense_grads_q8_workspace_bytes(dtype, M, K, N) || (work && aligned16(work)), 14,
+             "%s: work must be a 16-byte aligned device pointer", fn);
+  const GradsPlan p = grads_plan(M, K, N);
 #define GO2(T, R)                                                                                                       \
-  hipLaunchKernelGGL((dense_grads_q8_kernel<T, R>), grid, dim3(256), 0, (hipStream_t)stream, M, K, N,                 \
-                     (const uint8_t *)codes, (const uint8_t *)exps, (const T *)dY, lddy, dW, lddw, db)
+  launch_grads<T, R>((hipStream_t)stream, p, M, K, N, codes, exps, (const T *)dY, lddy, dW, lddw, db, (float *)work)
 #define GO(T) do { if (relu) GO2(T, true); else GO2(T, false); } while (0)
   LB_BY_DTYPE(dtype, GO);
 #undef GO

@@ -49,7 +49,7 @@ static inline SkinnyPlan skinny_plan(int64_t rows, int64_t L, int64_t O) {
 
 template <typename T, bool VJP, int RT>
 __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_t L, int64_t O, const T *__restrict__ X,
-                                                               int64_t ldx, const uint4 *__restrict__ codes,
+                                                               int64_t ldx, const u32x4 *__restrict__ codes,
                                                                const uint32_t *__restrict__ exps, int64_t Np, int64_t kbs,
                                                                int wk_n, int steps, int chunk, float *__restrict__ part,
                                                                Epilogue<T, VJP> ep) {
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
   const int wk = wave & (wk_n - 1), wn = wave / wk_n;
   const int c = lane >> 4, l16 = lane & 15;
   const int64_t tile = (int64_t)blockIdx.x * (SK_WAVES / wk_n) + wn;  // 32 outputs
-  const bool live = tile * 32 < O;
+  const int64_t o0 = (tile * 32 < O ? tile : (O - 1) / 32) * 32;           // a wave past the last tile repeats it, unused
   const int rows = P * (int)M;
   const int stride = chunk * 2 + 16;  // bytes of an image row: 16 more spread the rows over the banks
   const int64_t s_all = cdiv(L, 128), s_lo = (int64_t)blockIdx.y * steps;
@@ -68,26 +68,26 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
   if (VJP) tr.init(lane);
   const int lab = tr8_label(lane), half = l16 >> 3;
 
-  uint4 cw[2];       // codes of one step: 16 bytes for each of two columns, or 8 bytes for each of four
+  u32x2 cw[4];  // codes of one step: 16 bytes for each of two columns, or 8 bytes for each of four
   uint32_t ce[VJP ? 4 : 2];
   auto fetch = [&](int64_t s) {
+    // past the ends the last codes are read again: their outputs are unused, or they meet the image's zeros
     if (!VJP) {
-      const int64_t kb = 4 * s + c;
-      const bool in = live && s < s_hi && kb < kbs;
+      const int64_t kb = 4 * s + c < kbs ? 4 * s + c : kbs - 1;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int64_t n = tile * 32 + t * 16 + l16;
-        cw[t] = in ? codes[kb * Np + n] : make_uint4(0, 0, 0, 0);
-        ce[t] = in ? exps[kb * (Np / 8) + n / 8] : 0u;
+        const int64_t n = o0 + t * 16 + l16;
+        const u32x4 q = codes[kb * Np + n];
+        cw[2 * t] = u32x2{q.x, q.y};
+        cw[2 * t + 1] = u32x2{q.z, q.w};
+        ce[t] = exps[kb * (Np / 8) + n / 8];
       }
     } else {
-      uint2 *c2 = reinterpret_cast<uint2 *>(cw);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int64_t n0 = s * 128 + t * 32;
-        const bool in = live && s < s_hi && n0 < Np;
-        c2[t] = in ? reinterpret_cast<const uint2 *>(codes)[(tile * Np + n0 + c * 8 + lab) * 2 + half] : make_uint2(0, 0);
-        ce[t] = in ? exps[tile * (Np / 8) + n0 / 8 + c] : 0u;
+        const int64_t n0 = s * 128 + t * 32 < Np ? s * 128 + t * 32 : Np - 32;
+        cw[t] = reinterpret_cast<const u32x2 *>(codes)[(o0 / 32 * Np + n0 + c * 8 + lab) * 2 + half];
+        ce[t] = exps[o0 / 32 * (Np / 8) + n0 / 8 + c];
       }
     }
   };
@@ -118,37 +118,36 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
         Split<T>::two(v.v[2], v.v[3], b);
 #pragma unroll
         for (int p = 0; p < P; ++p)
-          *reinterpret_cast<uint2 *>(lds + (p * (int)M + m) * stride + k4 * 8) = make_uint2(a[p], b[p]);
+          *reinterpret_cast<u32x2 *>(lds + (p * (int)M + m) * stride + k4 * 8) = u32x2{a[p], b[p]};
       }
     }
     __syncthreads();
     for (int i = wk; i < chunk_steps; i += wk_n) {
       const int64_t s = s0 + i;
       if (s >= s_hi) break;
-      const uint4 w0 = cw[0], w1 = cw[1];
+      u32x2 w[4];
       uint32_t e[VJP ? 4 : 2];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) w[t] = cw[t];
 #pragma unroll
       for (int t = 0; t < (VJP ? 4 : 2); ++t) e[t] = ce[t];
       fetch(s + wk_n);
       const unsigned char *img = lds + i * 256;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint4 f0, f1;
+        u32x4 f0, f1;
         if (!VJP) {
-          const uint32_t d0 = j == 0 ? w0.x : j == 1 ? w0.y : j == 2 ? w0.z : w0.w;
-          const uint32_t d1 = j == 0 ? w1.x : j == 1 ? w1.y : j == 2 ? w1.z : w1.w;
+          const uint32_t d0 = j & 1 ? w[j >> 1].y : w[j >> 1].x, d1 = j & 1 ? w[2 + (j >> 1)].y : w[2 + (j >> 1)].x;
           f0 = w4_frag(d0, j == 0 ? w4_scale<0>(e[0]) : j == 1 ? w4_scale<1>(e[0]) : j == 2 ? w4_scale<2>(e[0]) : w4_scale<3>(e[0]));
           f1 = w4_frag(d1, j == 0 ? w4_scale<0>(e[1]) : j == 1 ? w4_scale<1>(e[1]) : j == 2 ? w4_scale<2>(e[1]) : w4_scale<3>(e[1]));
         } else {  // columns: row tiles 2 half and 2 half + 1 of the block of 32
-          const uint32_t d0 = j == 0 ? w0.x : j == 1 ? w0.z : j == 2 ? w1.x : w1.z;
-          const uint32_t d1 = j == 0 ? w0.y : j == 1 ? w0.w : j == 2 ? w1.y : w1.w;
           const uint32_t ej = e[VJP ? j : 0] >> (16 * half);
-          f0 = w4_frag(tr(d0), w4_scale<0>(ej));
-          f1 = w4_frag(tr(d1), w4_scale<1>(ej));
+          f0 = w4_frag(tr(w[j].x), w4_scale<0>(ej));
+          f1 = w4_frag(tr(w[j].y), w4_scale<1>(ej));
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const uint4 a = *reinterpret_cast<const uint4 *>(img + a_off[r] + (VJP ? j * 64 : j * 16));
+          const u32x4 a = *reinterpret_cast<const u32x4 *>(img + a_off[r] + (VJP ? j * 64 : j * 16));
           acc[r][0] = mfma(a, f0, acc[r][0]);
           acc[r][1] = mfma(a, f1, acc[r][1]);
         }
@@ -170,17 +169,31 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
         if (row < rows) red[(wave * rows + row) * 32 + o] = acc[r][t][v];
       }
   __syncthreads();
-  const int outs = SK_WAVES / wk_n * 32;
-  for (int i = tid; i < (int)M * outs; i += 64 * SK_WAVES) {
-    const int m = i / outs, oo = i - m * outs, w = oo >> 5, col = oo & 31;
-    const int64_t o = ((int64_t)blockIdx.x * (SK_WAVES / wk_n) + w) * 32 + col;
-    if (o >= O) continue;
-    float v = 0.0f;
+  // a thread keeps its output column (the columns of a workgroup divide its threads), four rows at a time
+  const int outs = SK_WAVES / wk_n * 32, oo = tid & (outs - 1), w = oo >> 5, col = oo & 31, dm = 64 * SK_WAVES / outs;
+  const int64_t o = ((int64_t)blockIdx.x * (SK_WAVES / wk_n) + w) * 32 + col;
+  if (o >= O) return;
+  const bool whole = gridDim.y == 1;
+  const float b = whole ? ep.bias_at(o) : 0.0f;
+  for (int m0 = tid / outs; m0 < (int)M; m0 += 4 * dm) {
+    float v[4];
+    uint32_t mask[4];
 #pragma unroll
-    for (int p = P - 1; p >= 0; --p)  // small pieces first
-      for (int k = 0; k < wk_n; ++k) v += red[((w * wk_n + k) * rows + p * (int)M + m) * 32 + col];
-    if (gridDim.y == 1) ep(m, o, v);
-    else part[((int64_t)blockIdx.y * M + m) * O + o] = v;
+    for (int u = 0; u < 4; ++u) mask[u] = m0 + u * dm < (int)M && whole ? ep.mask_at(m0 + u * dm, o) : 0u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      v[u] = 0.0f;
+      if (m0 + u * dm < (int)M)
+        for (int p = P - 1; p >= 0; --p)  // small pieces first
+          for (int k = 0; k < wk_n; ++k) v[u] += red[((w * wk_n + k) * rows + p * (int)M + m0 + u * dm) * 32 + col];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int m = m0 + u * dm;
+      if (m >= (int)M) break;
+      if (whole) ep.store(m, o, v[u], b, mask[u]);
+      else part[((int64_t)blockIdx.y * M + m) * O + o] = v[u];
+    }
   }
 }
 
@@ -191,7 +204,7 @@ static void launch_skinny(hipStream_t st, const SkinnyPlan &p, int64_t M, int64_
   const dim3 grid((unsigned)p.gx, (unsigned)p.splits);
 #define GO(RT)                                                                                                            \
   hipLaunchKernelGGL((skinny_kernel<T, VJP, RT>), grid, dim3(64 * SK_WAVES), 0, st, M, L, O, X, ldx,                    \
-                     (const uint4 *)codes, (const uint32_t *)exps, Np, kbs, p.wk, p.steps, p.chunk, part, ep)
+                     (const u32x4 *)codes, (const uint32_t *)exps, Np, kbs, p.wk, p.steps, p.chunk, part, ep)
   if (p.rt == 1) GO(1);
   else if (p.rt == 2) GO(2);
   else if (p.rt == 3) GO(3);

@@ -3,17 +3,17 @@
 // Bound by the matrix pipe (2 M K N flop per piece), so the loop must feed it: the floating operand is split into its
 // planes ONCE by split_planes_kernel (a workgroup splitting its own rows would repeat that for every 128 outputs, and
 // vector instructions compete with the matrix ones) and staged through LDS, double buffered, 64 reduction indices at a time,
-// 16-byte chunks at chunk ^ (row & 7) so that fragment reads and stage writes are free of bank conflicts; the codes go
+// 16-byte chunks at chunk ^ (row / 2 % 8) so that fragment reads and stage writes are free of bank conflicts; the codes go
 // straight from memory to registers, one step ahead, and are decoded where they are used.
 #pragma once
 #include "frag.hpp"
 
 namespace gpvae_lb {
 
-// planes[p][m][Lp] of X [M, ldx], zero past L (Lp a multiple of 64)
+// planes[p][k / 64][m][k % 64] of X [M, ldx], zero past L (Lp a multiple of 64): what a step stages is contiguous
 template <typename T>
 __global__ __launch_bounds__(256) void split_planes_kernel(int64_t M, int64_t L, int64_t Lp, const T *__restrict__ X, int64_t ldx,
-                                                           uint2 *__restrict__ planes) {
+                                                           u32x2 *__restrict__ planes) {
   constexpr int P = Split<T>::P;
   const int64_t q = Lp / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= M * q) return;
@@ -23,66 +23,91 @@ __global__ __launch_bounds__(256) void split_planes_kernel(int64_t M, int64_t L,
   Split<T>::two(v.v[0], v.v[1], a);
   Split<T>::two(v.v[2], v.v[3], b);
 #pragma unroll
-  for (int p = 0; p < P; ++p) planes[p * M * q + i] = make_uint2(a[p], b[p]);
+  for (int p = 0; p < P; ++p) planes[p * M * q + ((k4 >> 4) * M + m) * 16 + (k4 & 15)] = u32x2{a[p], b[p]};
 }
 
 // WM x 2 waves, each 16 MT rows x 64 outputs
+// Addresses are a scalar base that moves with the step plus a fixed 32-bit offset per lane, so that the loop spends no vector
+// instruction on them.  Operand element (piece p, row m, reduction index k) is at byte p ps + (k / 64) ss + m rs + 2 (k % 64).
 template <typename T, bool VJP, int WM, int MT>
-__global__ __launch_bounds__(128 * WM, WM == 4 ? 2 : 3) void tile_kernel(int64_t M, int64_t Lp, int64_t O, const uint16_t *__restrict__ planes,
-                                                           int64_t ldp, int64_t plane, const uint4 *__restrict__ codes,
-                                                           const uint32_t *__restrict__ exps, int64_t Np, int64_t kbs, int mtiles,
-                                                           int steps, float *__restrict__ part, Epilogue<T, VJP> ep) {
+__global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O, const char *__restrict__ planes, int64_t rs,
+                                                           int64_t ss, int64_t ps, const char *__restrict__ codes,
+                                                           const char *__restrict__ exps, int64_t Np, int64_t kbs, int mtiles,
+                                                           int64_t s_all, int steps, float *__restrict__ part,
+                                                           Epilogue<T, VJP> ep) {
   constexpr int P = Split<T>::P, NT = 128 * WM, BM = 16 * MT * WM;
   constexpr int CH = P * BM * 8, NLD = CH / NT;  // 16-byte chunks of a stage, and of one thread's share
-  static_assert(CH % NT == 0, "whole shares");
+  static_assert(BM % (NT / 8) == 0 && NT / 8 % 8 == 0, "whole shares");
   __shared__ __align__(16) unsigned char lds[2][CH * 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wo = wave & 1, c = lane >> 4, l16 = lane & 15;
   const int64_t bt = blockIdx.x, m0 = (bt % mtiles) * BM, o0 = (bt / mtiles) * 128 + wo * 64;  // row tiles fastest
-  const int64_t s_all = Lp / 64, s_lo = (int64_t)blockIdx.y * steps;
-  const int64_t s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
+  const int64_t s_lo = (int64_t)blockIdx.y * steps, s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
   Tr8 tr;
   if (VJP) tr.init(lane);
   const int lab = tr8_label(lane), half = l16 >> 3;
 
-  // stage share: chunk id -> (piece, row, 16-byte chunk)
-  uint4 st[NLD];
-  const uint16_t *src[NLD];
-  int dst[NLD];
+  // stage share: thread -> 16-byte chunk tid % 8 of rows tid / 8 + RP i of every plane
+  constexpr int RP = NT / 8, NR = BM / RP;
+  const int ck8 = tid & 7, trow = tid >> 3;
+  uint32_t src[NR];
 #pragma unroll
-  for (int i = 0; i < NLD; ++i) {
-    const int id = i * NT + tid, ck = id & 7, row = (id >> 3) % BM, p = (id >> 3) / BM;
-    const int64_t m = m0 + row < M ? m0 + row : M - 1;  // rows past the last: results unused
-    src[i] = planes + p * plane + m * ldp + ck * 8;
-    dst[i] = ((p * BM + row) * 8 + (ck ^ (row & 7))) * 16;
+  for (int i = 0; i < NR; ++i) {
+    const int64_t row = trow + i * RP;
+    src[i] = (uint32_t)((m0 + row < M ? row : M - 1 - m0) * rs) + ck8 * 16;  // rows past the last: results unused
   }
-  auto stage_load = [&](int64_t s) {
-#pragma unroll
-    for (int i = 0; i < NLD; ++i) st[i] = *reinterpret_cast<const uint4 *>(src[i] + s * 64);
-  };
-  auto stage_store = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < NLD; ++i) *reinterpret_cast<uint4 *>(lds[b] + dst[i]) = st[i];
-  };
+  const char *const pbase = planes + m0 * rs;
+  const int dst = (trow * 8 + (ck8 ^ ((trow >> 1) & 7))) * 16;
   // codes of one step: product: 8 bytes (two groups of 8 rows) of each of 4 columns 16 apart, lane group c taking rows
-  // 32 (c / 2) + 16 (c % 2) + ...; transposed product: 8 bytes of a column for two blocks of 32 columns x two of 32 rows
-  uint2 cw[4];
-  uint32_t ce[4];
-  auto fetch = [&](int64_t s) {
+  // 32 (c / 2) + 16 (c % 2) + ...; transposed product: 8 bytes of a column for two blocks of 32 columns x two of 32 rows.
+  // Past the ends the last codes are read again: their outputs are unused, or they meet the operand's zeros.
+  uint32_t coff[4], eoff[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if (!VJP) {
-        const int64_t kb = 2 * s + (c >> 1), n = o0 + t * 16 + l16;
-        const bool in = kb < kbs && n < Np;
-        cw[t] = in ? reinterpret_cast<const uint2 *>(codes)[(kb * Np + n) * 2 + (c & 1)] : make_uint2(0, 0);
-        ce[t] = in ? exps[kb * (Np / 8) + n / 8] >> (16 * (c & 1)) : 0u;
-      } else {
-        const int64_t n = s * 64 + (t >> 1) * 32, kb = o0 / 32 + (t & 1);
-        const bool in = n < Np && kb < kbs;
-        cw[t] = in ? reinterpret_cast<const uint2 *>(codes)[(kb * Np + n + c * 8 + lab) * 2 + half] : make_uint2(0, 0);
-        ce[t] = in ? exps[kb * (Np / 8) + n / 8 + c] >> (16 * half) : 0u;
+  for (int t = 0; t < 4; ++t) {
+    if (!VJP) {
+      const int64_t n = o0 + t * 16 + l16 < Np ? o0 + t * 16 + l16 : Np - 1;
+      coff[t] = (uint32_t)(((c >> 1) * Np + n) * 16 + (c & 1) * 8);
+      eoff[t] = (uint32_t)(((c >> 1) * (Np / 8) + n / 8) * 4);
+    } else {
+      coff[t] = ((t >> 1) * 32 + c * 8 + lab) * 16 + half * 8;
+      eoff[t] = ((t >> 1) * 4 + c) * 4;
+    }
+  }
+  const int64_t kbv0 = VJP ? (o0 / 32 < kbs ? o0 / 32 : kbs - 1) : 0, kbv1 = VJP ? (o0 / 32 + 1 < kbs ? o0 / 32 + 1 : kbs - 1) : 0;
+  struct Ahead {  // what is in flight for a step: its share of the stage, its codes and tile exponents
+    u32x4 st[NLD];
+    u32x2 cw[4];
+    uint32_t ce[4];
+  };
+  auto issue = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
+    if (s >= s_hi) return;
+    const char *const b = pbase + s * ss;
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) h.st[i] = *reinterpret_cast<const u32x4 *>(b + (i / NR) * ps + src[i % NR]);
+    if (!VJP) {
+      const char *const cb = codes + 2 * s * Np * 16, *const eb = exps + 2 * s * (Np / 2);
+      const bool odd = 2 * s + 1 >= kbs;  // the last block has no second one: lane groups 2, 3 read the first again
+      const uint32_t back_c = odd && c >= 2 ? (uint32_t)(Np * 16) : 0u, back_e = odd && c >= 2 ? (uint32_t)(Np / 2) : 0u;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        h.cw[t] = *reinterpret_cast<const u32x2 *>(cb + (coff[t] - back_c));
+        h.ce[t] = *reinterpret_cast<const uint32_t *>(eb + (eoff[t] - back_e));
+      }
+    } else {
+      // columns 64 s + 32 (t / 2) ...: a second half past the end repeats the first
+      const uint32_t back = s * 64 + 32 >= Np ? 32u : 0u;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int64_t kb = t & 1 ? kbv1 : kbv0;
+        const uint32_t bk = t >> 1 ? back : 0u;
+        h.cw[t] = *reinterpret_cast<const u32x2 *>(codes + (kb * Np + s * 64) * 16 + (coff[t] - bk * 16));
+        h.ce[t] = *reinterpret_cast<const uint32_t *>(exps + (kb * Np + s * 64) / 2 + (eoff[t] - bk / 2));
       }
     }
+  };
+  auto put = [&](const Ahead &h, int b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NLD; ++i) *reinterpret_cast<u32x4 *>(lds[b] + dst + i * RP * 128) = h.st[i];
   };
 
   f32x4_t acc[MT][4];
@@ -90,57 +115,96 @@ __global__ __launch_bounds__(128 * WM, WM == 4 ? 2 : 3) void tile_kernel(int64_t
   for (int a = 0; a < MT; ++a)
 #pragma unroll
     for (int b = 0; b < 4; ++b) acc[a][b] = f32x4_t{0, 0, 0, 0};
-  stage_load(s_lo);
-  fetch(s_lo);
-  stage_store(0);
-  __syncthreads();
-  const int arow = (wm * MT * 16 + l16) * 128, sw = l16 & 7;
-  for (int64_t s = s_lo; s < s_hi; ++s) {
-    const int b = (int)(s - s_lo) & 1;
-    const uint2 w[4] = {cw[0], cw[1], cw[2], cw[3]};
-    const uint32_t e[4] = {ce[0], ce[1], ce[2], ce[3]};
-    const bool more = s + 1 < s_hi;
-    if (more) {
-      stage_load(s + 1);
-      fetch(s + 1);
-    }
+  const int arow = (wm * MT * 16 + l16) * 128, sw = l16 >> 1;
+  // one step: codes of step s in `now`, its stage in lds[b]; `next` holds step s + 1 in flight, step s + 2 replaces `now`
+  auto step = [&](Ahead &now, Ahead &next, int64_t s, int b) __attribute__((always_inline)) {
+    u32x2 w[4];
+    uint32_t e[4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      uint4 f[4];
-      if (!VJP) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = w4_frag(t ? w[i].y : w[i].x, t ? w4_scale<1>(e[i]) : w4_scale<0>(e[i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          f[2 * i] = w4_frag(tr(w[2 * t + i].x), w4_scale<0>(e[2 * t + i]));
-          f[2 * i + 1] = w4_frag(tr(w[2 * t + i].y), w4_scale<1>(e[2 * t + i]));
-        }
-      }
+    for (int t = 0; t < 4; ++t) w[t] = now.cw[t], e[t] = now.ce[t] >> (16 * (VJP ? half : c & 1));
+    u32x4 x[2][P][MT], f[2][4];
+    auto read = [&](int t) __attribute__((always_inline)) {
       const int ck = ((VJP ? t * 4 + c : 2 * c + t) ^ sw) * 16;
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-        for (int a = 0; a < MT; ++a) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(lds[b] + p * BM * 128 + arow + a * 2048 + ck);
+        for (int a = 0; a < MT; ++a) x[t][p][a] = *reinterpret_cast<const u32x4 *>(lds[b] + p * BM * 128 + arow + a * 2048 + ck);
+    };
+    auto decode = [&](int t) __attribute__((always_inline)) {
+      if (!VJP) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[a][i] = mfma(x, f[i], acc[a][i]);
+        for (int i = 0; i < 4; ++i) f[t][i] = w4_frag(t ? w[i].y : w[i].x, t ? w4_scale<1>(e[i]) : w4_scale<0>(e[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          f[t][2 * i] = w4_frag(tr(w[2 * t + i].x), w4_scale<0>(e[2 * t + i]));
+          f[t][2 * i + 1] = w4_frag(tr(w[2 * t + i].y), w4_scale<1>(e[2 * t + i]));
         }
+      }
+    };
+    auto multiply = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int p = P - 1; p >= 0; --p)
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[a][i] = mfma(x[t][p][a], f[t][i], acc[a][i]);
+    };
+    // the compiler alone reads two fragments, waits, multiplies, and so on: all of a half step's fragments are read before
+    // the previous half is multiplied, and its decoding runs between that half's matrix instructions
+    read(0);
+    issue(now, s + 2);
+    decode(0);
+    __builtin_amdgcn_sched_barrier(0);
+    read(1);
+    __builtin_amdgcn_sched_barrier(0);
+    decode(1);
+    multiply(0);
+#pragma unroll
+    for (int i = 0; i < P * MT * 4; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one matrix instruction
+      __builtin_amdgcn_sched_group_barrier(0x002, VJP ? 4 : 2, 0);  // vector instructions
     }
-    if (more) stage_store(b ^ 1);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(1);
+    if (s + 1 < s_hi) put(next, b ^ 1);
     __syncthreads();
+  };
+  Ahead h0, h1;
+  issue(h0, s_lo);
+  issue(h1, s_lo + 1);
+  put(h0, 0);
+  __syncthreads();
+  for (int64_t s = s_lo; s < s_hi; s += 2) {
+    step(h0, h1, s, 0);
+    if (s + 1 < s_hi) step(h1, h0, s + 1, 1);
+  }
+  const bool whole = gridDim.y == 1;
+  int64_t oi[4];
+  float bv[4];
+  uint32_t mask[MT][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    oi[i] = o0 + (VJP ? (i >> 1) * 32 + (2 * half + (i & 1)) * 8 + lab : i * 16 + l16);
+    const int64_t oc = oi[i] < O ? oi[i] : O - 1;
+    bv[i] = whole ? ep.bias_at(oc) : 0.0f;
+#pragma unroll
+    for (int a = 0; a < MT; ++a) {
+      const int64_t m = m0 + (wm * MT + a) * 16 + 4 * c;
+      mask[a][i] = whole ? ep.mask4_at(m < M ? m : 0, oc) : 0u;
+    }
   }
 #pragma unroll
   for (int a = 0; a < MT; ++a)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t o = o0 + (VJP ? (i >> 1) * 32 + (2 * half + (i & 1)) * 8 + lab : i * 16 + l16);
+    for (int r = 0; r < 4; ++r) {
+      const int64_t m = m0 + (wm * MT + a) * 16 + 4 * c + r;
+      if (m >= M) continue;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t m = m0 + (wm * MT + a) * 16 + 4 * c + r;
-        if (m >= M || o >= O) continue;
-        if (gridDim.y == 1) ep(m, o, acc[a][i][r]);
-        else part[((int64_t)blockIdx.y * M + m) * O + o] = acc[a][i][r];
+      for (int i = 0; i < 4; ++i) {
+        if (oi[i] >= O) continue;
+        if (whole) ep.store(m, oi[i], acc[a][i][r], bv[i], (mask[a][i] >> (8 * r)) & 255u);
+        else part[((int64_t)blockIdx.y * M + m) * O + oi[i]] = acc[a][i][r];
       }
     }
 }
@@ -155,7 +219,7 @@ struct TilePlan {
 static inline TilePlan tile_plan(int P, int64_t M, int64_t L, int64_t O, bool direct) {
   TilePlan p;
   p.direct = direct;
-  p.wm = M <= 64 ? 2 : 4;
+  p.wm = 2;
   p.mt = 2;
   p.Lp = round_up(L, 64);
   p.mtiles = (int)cdiv(M, 16 * p.mt * p.wm);
@@ -174,20 +238,19 @@ template <typename T, bool VJP>
 static void launch_tile(hipStream_t st, const TilePlan &p, int64_t M, int64_t L, int64_t O, const T *X, int64_t ldx,
                         const void *codes, const void *exps, int64_t Np, int64_t kbs, unsigned char *work,
                         const Epilogue<T, VJP> &ep) {
-  const uint16_t *planes = reinterpret_cast<const uint16_t *>(X);
-  int64_t ldp = ldx, plane = 0;
+  const char *planes = reinterpret_cast<const char *>(X);
+  int64_t rs = ldx * 2, ss = 128, ps = 0;
   if (!p.direct) {
     hipLaunchKernelGGL((split_planes_kernel<T>), dim3((unsigned)cdiv(M * p.Lp / 4, 256)), dim3(256), 0, st, M, L, p.Lp, X, ldx,
-                       (uint2 *)work);
-    planes = reinterpret_cast<const uint16_t *>(work);
-    ldp = p.Lp;
-    plane = M * p.Lp;
+                       (u32x2 *)work);
+    planes = reinterpret_cast<const char *>(work);
+    rs = 128, ss = M * 128, ps = M * p.Lp * 2;
   }
   float *part = reinterpret_cast<float *>(work + p.plane_bytes);
   const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
 #define GO(WM, MT)                                                                                                        \
-  hipLaunchKernelGGL((tile_kernel<T, VJP, WM, MT>), grid, dim3(128 * WM), 0, st, M, p.Lp, O, planes, ldp, plane,        \
-                     (const uint4 *)codes, (const uint32_t *)exps, Np, kbs, p.mtiles, p.steps, part, ep)
+  hipLaunchKernelGGL((tile_kernel<T, VJP, WM, MT>), grid, dim3(128 * WM), 0, st, M, O, planes, rs, ss, ps,              \
+                     (const char *)codes, (const char *)exps, Np, kbs, p.mtiles, p.Lp / 64, p.steps, part, ep)
   if (p.wm == 2) GO(2, 2);
   else GO(4, 2);
 #undef GO

@@ -49,8 +49,9 @@ __global__ __launch_bounds__(256) void load_w4_kernel(int64_t K, int64_t N, cons
 
 static int check_w4(const char *fn, int dtype, int64_t K, int64_t N, int kn_arg) {
   LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
+  // N: two rows of code words lie within a 32-bit offset
   LB_REQUIRE(K >= 1 && K <= (1 << 30), kn_arg, "%s: K must lie in [1, 2^30] (got %lld)", fn, (long long)K);
-  LB_REQUIRE(N >= 1 && N <= (1 << 30), kn_arg + 1, "%s: N must lie in [1, 2^30] (got %lld)", fn, (long long)N);
+  LB_REQUIRE(N >= 1 && N <= (1 << 26), kn_arg + 1, "%s: N must lie in [1, 2^26] (got %lld)", fn, (long long)N);
   return 0;
 }
 
@@ -114,8 +115,9 @@ static void run_w4(hipStream_t st, int64_t M, int64_t L, int64_t O, const void *
   if (P * M <= SK_MAXROWS) {
     launch_skinny<T, VJP>(st, skinny_plan(P * M, L, O), M, L, O, (const T *)X, ldx, codes, exps, Np, kbs, (float *)work, ep);
   } else {
-    // a bfloat16 operand is its own plane where its rows can be read 16 bytes at a time to the end of the last step
-    const bool direct = P == 1 && L % 64 == 0 && ldx % 8 == 0 && aligned16(X);
+    // a bfloat16 operand is its own plane where its rows can be read 16 bytes at a time to the end of the last step and
+    // 256 of them lie within a 32-bit offset
+    const bool direct = P == 1 && L % 64 == 0 && ldx % 8 == 0 && ldx < (1 << 23) && aligned16(X);
     launch_tile<T, VJP>(st, tile_plan(P, M, L, O, direct), M, L, O, (const T *)X, ldx, codes, exps, Np, kbs,
                         (unsigned char *)work, ep);
   }
