@@ -14,6 +14,12 @@ __device__ __forceinline__ f32x4_t mfma(u32x4 a, u32x4 b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
+// Workgroups are dealt to the 8 XCDs round-robin; this renumbers them so that an XCD gets a contiguous run.
+__device__ __forceinline__ int64_t xcd_chunk(int64_t id, int64_t n) {
+  const int64_t x = id & 7, q = n >> 3, r = n & 7;
+  return x * q + (x < r ? x : r) + (id >> 3);
+}
+
 // ---- w4 -----------------------------------------------------------------------------------------------------------------
 // 8 codes -> 8 bfloat16 values; byte J of the tile-exponent word e is their exponent
 template <int J> __device__ __forceinline__ float w4_scale(uint32_t e) {

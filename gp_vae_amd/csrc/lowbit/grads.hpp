@@ -6,7 +6,8 @@
 // LDS: a thread loads 8 consecutive rows of a column (consecutive lanes: consecutive columns), splits them into their
 // bfloat16 pieces and writes each piece's 8 values as 16 bytes.  Bound by the matrix pipe and LDS (one 128 x 128
 // tile per workgroup, 64 rows a step): the conversions are vector work that is dealt between the matrix instructions of
-// the step before.
+// the step before.  All row tiles of a column tile run on one XCD (xcd_chunk), whose L2 then serves dY to them: dealt
+// round-robin every XCD read all of dY from memory (4096 x 1024 x 4096 float32: 140 us; with it see the launch).
 #pragma once
 #include "frag.hpp"
 
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   __shared__ __align__(16) unsigned char lds[2][ST];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave >> 2, wn = wave & 3, c = lane >> 4, l16 = lane & 15;  // wave: 64 rows of dW x 32 columns
-  const int64_t bt = blockIdx.x, kt = bt % ktiles, k0 = kt * 128, n0 = (bt / ktiles) * 128;
+  const int64_t bt = xcd_chunk(blockIdx.x, gridDim.x), kt = bt % ktiles, k0 = kt * 128, n0 = (bt / ktiles) * 128;
   const int64_t s_lo = (int64_t)blockIdx.y * steps, s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
   const int64_t Kp = q8_kp(K), mbs = q8_mb(M);
   const bool sum_db = db != nullptr && kt == 0;
@@ -78,29 +79,33 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
     u32x2 q[2];
     uint32_t e[2];
   };
+  // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
+  // may not have been issued does not count, so that the wait would reach into the step just issued.  Past the last step
+  // and the last row the last ones are read again.
   auto issue = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
-    if (s >= s_hi) return;
+    s = s < s_hi ? s : s_hi - 1;
     const int64_t m = s * GR_ROWS + wave * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (m + i < M) {
-        const char *row = reinterpret_cast<const char *>(dY + (m + i) * lddy + n0);
+      const char *row = reinterpret_cast<const char *>(dY + (m + i < M ? m + i : M - 1) * lddy + n0);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) h.y[i][e] = *reinterpret_cast<const T *>(row + yoff[e]);
-      } else {  // rows past the last add nothing
-        h.y[i][0] = h.y[i][1] = T(0.0f);
-      }
+      for (int e = 0; e < 2; ++e) h.y[i][e] = *reinterpret_cast<const T *>(row + yoff[e]);
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       int64_t mb = s * (GR_ROWS / 8) + xb + 4 * j;
-      mb = mb < mbs ? mb : mbs - 1;  // finite (or already NaN) times the zeros above
+      mb = mb < mbs ? mb : mbs - 1;  // finite (or already NaN) times the zeros that put makes of rows past the last
       h.q[j] = *reinterpret_cast<const u32x2 *>(codes + (mb * Kp + k0) * 8 + xoff);
       h.e[j] = (exps + mb * (Kp / 8) + k0 / 8)[eoff];
     }
   };
   float dbacc[2] = {0.0f, 0.0f};
-  auto put = [&](const Ahead &h, int b) __attribute__((always_inline)) {
+  auto put = [&](Ahead &h, int64_t s, int b) __attribute__((always_inline)) {
+    if ((s + 1) * GR_ROWS > M) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (s * GR_ROWS + wave * 8 + i >= M) h.y[i][0] = h.y[i][1] = T(0.0f);
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       uint32_t w[4][P];
@@ -113,7 +118,7 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       *reinterpret_cast<u32x4 *>(lds[b] + xk * 128 + (((xb + 4 * j) ^ xsw) * 16)) = q8_frag<RELU>(h.q[j], h.e[j]);
-    if (sum_db) {
+    if (sum_db && s < s_hi) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -148,14 +153,14 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
         for (int a = 0; a < 4; ++a)
 #pragma unroll
           for (int i = 0; i < 2; ++i) acc[a][i] = mfma(x[t][a], y[t][p][i], acc[a][i]);
-    if (s + 1 < s_hi) put(next, b ^ 1);
+    put(next, s + 1, b ^ 1);
     __syncthreads();
   };
   Ahead h0, h1;
   if (s_lo < s_hi) {
     issue(h0, s_lo);
     issue(h1, s_lo + 1);
-    put(h0, 0);
+    put(h0, s_lo, 0);
   }
   __syncthreads();
   for (int64_t s = s_lo; s < s_hi; s += 2) {

@@ -3,54 +3,116 @@
 
 namespace gpvae_lb {
 
-// One thread per tile of 8 x 8.
+// Bound by memory: X is read once, Y and the codes are written once.  A thread owns a strip of 8 rows x 4 columns, half a
+// tile: 8 loads of 4 elements (16 bytes of float32) cover the strip, the tile's largest magnitude is one exchange with the
+// neighbouring lane, and its 4 columns of codes are 32 consecutive bytes.  Consecutive lanes take consecutive
+// strips of the same rows, so that every row of a wave is one contiguous stretch.
 template <typename T, bool RELU>
 __global__ __launch_bounds__(256) void store_q8_kernel(int64_t M, int64_t K, const T *X, int64_t ldx, T *Y, int64_t ldy,
                                                        uint8_t *__restrict__ codes, uint8_t *__restrict__ exps) {
-  const int64_t Kp = q8_kp(K), kt = Kp / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= q8_mb(M) * kt) return;
-  const int64_t mb = id / kt, t = id % kt, m0 = mb * 8, k0 = t * 8;
-  float amax = 0.0f;
-  bool bad = false;
-  for (int i = 0; i < 8; ++i)
-    for (int c = 0; c < 8; ++c)
-      if (m0 + i < M && k0 + c < K) {
-        float v = to_f32(X[(m0 + i) * ldx + k0 + c]);
-        if (RELU) v = v < 0.0f ? 0.0f : v;
-        bad |= !(fabsf(v) <= 3.402823466e+38f);
-        amax = fmaxf(amax, fabsf(v));
-      }
-  const int eb = bad ? 255 : (RELU ? tile_exp_byte<255, 7, -126>(amax) : tile_exp_byte<127, 6, -126>(amax));
-  exps[mb * kt + t] = (uint8_t)eb;
-  for (int c = 0; c < 8; ++c) {
-    uint64_t w = 0;
+  const int64_t Kp = q8_kp(K), strips = Kp / 4, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t all = q8_mb(M) * strips;
+  const bool live = id < all;  // (an even number of strips: a pair of lanes is live or not together)
+  const int64_t mb = live ? id / strips : 0, k0 = live ? (id - mb * strips) * 4 : 0, m0 = mb * 8;
+  const bool whole = m0 + 8 <= M && k0 + 4 <= K;
+  Vec4<T> v[8];
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const Vec4<T> *>(X + (m0 + i) * ldx + k0);
+  } else {
+#pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (m0 + i < M && k0 + c < K) {
-        float v = to_f32(X[(m0 + i) * ldx + k0 + c]);
-        if (RELU) {
-          v = v < 0.0f ? 0.0f : v;
-          if (Y) Y[(m0 + i) * ldy + k0 + c] = from_f32<T>(v);
-        }
-        int q = bad ? 0 : (int)rintf(unscale<RELU ? 255 : 127>(v, eb));
-        if (RELU && q == 0 && !(v <= 0.0f)) q = 1;
-        w |= (uint64_t)(uint8_t)q << (8 * i);
-      }
-    *reinterpret_cast<uint64_t *>(codes + (mb * Kp + k0 + c) * 8) = w;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[i].v[c] = live && m0 + i < M && k0 + c < K ? X[(m0 + i) * ldx + k0 + c] : T(0.0f);
   }
+  if (RELU) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[i].v[c] = to_f32(v[i].v[c]) < 0.0f ? T(0.0f) : v[i].v[c];
+    if (Y) {
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<Vec4<T> *>(Y + (m0 + i) * ldy + k0) = v[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (live && m0 + i < M && k0 + c < K) Y[(m0 + i) * ldy + k0 + c] = v[i].v[c];
+      }
+    }
+  }
+  // the largest magnitude as bits: an infinity or a NaN is above every finite value
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t b = __builtin_bit_cast(uint32_t, to_f32(v[i].v[c])) & 0x7fffffffu;
+      top = b > top ? b : top;
+    }
+  const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true);  // the lane next to it
+  const float amax = __builtin_bit_cast(float, other > top ? other : top);
+  const int eb = RELU ? tile_exp_byte<255, 7, -126>(amax) : tile_exp_byte<127, 6, -126>(amax);
+  const int e = eb - 127, h = e >> 1;
+  const float s1 = pow2f(-h), s2 = pow2f(h - e);
+  uint32_t w[4][2];
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      w[c][g] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = to_f32(v[4 * g + i].v[c]);
+        uint32_t q = 0;
+        if (RELU) {
+          q = (uint32_t)fminf(rintf(x * s1 * s2), 255.0f);
+          q = eb == 255 ? 0u : q;
+          q = q == 0 && !(x <= 0.0f) ? 1u : q;
+        } else {
+          q = (uint32_t)(int)fminf(fmaxf(rintf(x * s1 * s2), -127.0f), 127.0f) & 255u;
+          q = eb == 255 ? 0u : q;
+        }
+        w[c][g] |= q << (8 * i);
+      }
+    }
+  if (!live) return;
+  u32x4 *dst = reinterpret_cast<u32x4 *>(codes + (mb * Kp + k0) * 8);
+  dst[0] = u32x4{w[0][0], w[0][1], w[1][0], w[1][1]};
+  dst[1] = u32x4{w[2][0], w[2][1], w[3][0], w[3][1]};
+  if ((id & 1) == 0) exps[mb * (Kp / 8) + k0 / 8] = (uint8_t)eb;
 }
 
-template <bool RELU>
-__device__ __forceinline__ float q8_value(const uint8_t *codes, const uint8_t *exps, int64_t Kp, int64_t m, int64_t k) {
-  const uint8_t q = codes[((m / 8) * Kp + k) * 8 + m % 8];
-  return (RELU ? (float)q : (float)(int8_t)q) * scale_of(exps[(m / 8) * (Kp / 8) + k / 8]);
-}
-
+// The reverse: a thread reads its strip's 32 bytes of codes and writes 8 rows of 4 elements.
 template <typename T, bool RELU>
 __global__ __launch_bounds__(256) void load_q8_kernel(int64_t M, int64_t K, const uint8_t *__restrict__ codes,
                                                       const uint8_t *__restrict__ exps, T *__restrict__ out, int64_t ldo) {
-  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (k >= K) return;
-  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) out[m * ldo + k] = from_f32<T>(q8_value<RELU>(codes, exps, q8_kp(K), m, k));
+  const int64_t Kp = q8_kp(K), strips = Kp / 4, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= q8_mb(M) * strips) return;
+  const int64_t mb = id / strips, k0 = (id - mb * strips) * 4, m0 = mb * 8;
+  const u32x4 *src = reinterpret_cast<const u32x4 *>(codes + (mb * Kp + k0) * 8);
+  const u32x4 a = src[0], b = src[1];
+  const uint32_t w[4][2] = {{a.x, a.y}, {a.z, a.w}, {b.x, b.y}, {b.z, b.w}};
+  const float s = scale_of(exps[mb * (Kp / 8) + k0 / 8]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    Vec4<T> v;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t q = (w[c][i >> 2] >> (8 * (i & 3))) & 255u;
+      v.v[c] = from_f32<T>((RELU ? (float)q : (float)(int8_t)q) * s);
+    }
+    if (m0 + i >= M) break;
+    if (k0 + 4 <= K) {
+      *reinterpret_cast<Vec4<T> *>(out + (m0 + i) * ldo + k0) = v;
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (k0 + c < K) out[(m0 + i) * ldo + k0 + c] = v.v[c];
+    }
+  }
 }
 
 static int check_q8(const char *fn, int dtype, int64_t M, int64_t K) {
@@ -76,10 +138,10 @@ extern "C" int gpvae_store_q8(void *stream, int dtype, int64_t M, int64_t K, con
   LB_REQUIRE(Y != X || ldy == ldx, 9, "%s: in place needs ldy == ldx", fn);
   LB_REQUIRE(codes && aligned16(codes), 10, "%s: codes must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(exps && aligned16(exps), 11, "%s: exps must be a 16-byte aligned device pointer", fn);
-  const int64_t tiles = q8_mb(M) * (q8_kp(K) / 8);
-  LB_REQUIRE(cdiv(tiles, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+  const int64_t strips = q8_mb(M) * (q8_kp(K) / 4);
+  LB_REQUIRE(cdiv(strips, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
 #define GO2(T, R)                                                                                                        \
-  hipLaunchKernelGGL((store_q8_kernel<T, R>), dim3((unsigned)cdiv(tiles, 256)), dim3(256), 0, (hipStream_t)stream, M, K, \
+  hipLaunchKernelGGL((store_q8_kernel<T, R>), dim3((unsigned)cdiv(strips, 256)), dim3(256), 0, (hipStream_t)stream, M, K, \
                      (const T *)X, ldx, (T *)Y, ldy, (uint8_t *)codes, (uint8_t *)exps)
 #define GO(T) do { if (relu) GO2(T, true); else GO2(T, false); } while (0)
   LB_BY_DTYPE(dtype, GO);
@@ -98,7 +160,9 @@ extern "C" int gpvae_load_q8(void *stream, int dtype, int64_t M, int64_t K, int 
   LB_REQUIRE(exps && aligned16(exps), 7, "%s: exps must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(out, 8, "%s: out is NULL", fn);
   LB_REQUIRE(ldo >= K, 9, "%s: ldo < K", fn);
-  const dim3 grid((unsigned)cdiv(K, 256), (unsigned)(M < 65535 ? M : 65535));
+  const int64_t strips = q8_mb(M) * (q8_kp(K) / 4);
+  LB_REQUIRE(cdiv(strips, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+  const dim3 grid((unsigned)cdiv(strips, 256));
 #define GO2(T, R)                                                                                                  \
   hipLaunchKernelGGL((load_q8_kernel<T, R>), grid, dim3(256), 0, (hipStream_t)stream, M, K, (const uint8_t *)codes, \
                      (const uint8_t *)exps, (T *)out, ldo)

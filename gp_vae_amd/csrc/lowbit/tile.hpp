@@ -79,8 +79,11 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
     u32x2 cw[4];
     uint32_t ce[4];
   };
+  // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
+  // may not have been issued does not count, so that the wait would reach into the step just issued.  Past the last step
+  // the last one is read again.
   auto issue = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
-    if (s >= s_hi) return;
+    s = s < s_hi ? s : s_hi - 1;
     const char *const b = pbase + s * ss;
 #pragma unroll
     for (int i = 0; i < NLD; ++i) h.st[i] = *reinterpret_cast<const u32x4 *>(b + (i / NR) * ps + src[i % NR]);
@@ -167,7 +170,7 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
     }
     __builtin_amdgcn_sched_barrier(0);
     multiply(1);
-    if (s + 1 < s_hi) put(next, b ^ 1);
+    put(next, b ^ 1);
     __syncthreads();
   };
   Ahead h0, h1;

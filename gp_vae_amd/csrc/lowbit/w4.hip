@@ -4,47 +4,89 @@
 
 namespace gpvae_lb {
 
-// One thread per tile of 8 x 8.
+// Bound by memory: W is read once.  A thread owns 32 rows x 4 columns, half of four tiles: rows are read 4 elements at a time
+// (consecutive lanes: consecutive columns), a tile's largest magnitude is one exchange with the neighbouring lane, and
+// the codes of its 4 columns are 64 consecutive bytes.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_w4_kernel(int64_t K, int64_t N, const T *__restrict__ W, int64_t ldw,
-                                                       uint32_t *__restrict__ codes, uint8_t *__restrict__ exps) {
-  const int64_t Np = w4_np(N), nt = Np / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= w4_kb(K) * 4 * nt) return;
-  const int64_t t = id % nt, kt = id / nt, k0 = kt * 8, n0 = t * 8;
-  float amax = 0.0f;
-  bool bad = false;
-  for (int i = 0; i < 8; ++i)
-    for (int c = 0; c < 8; ++c)
-      if (k0 + i < K && n0 + c < N) {
-        const float a = fabsf(to_f32(W[(k0 + i) * ldw + n0 + c]));
-        bad |= !(a <= 3.402823466e+38f);
-        amax = fmaxf(amax, a);
+                                                       u32x4 *__restrict__ codes, uint32_t *__restrict__ exps) {
+  const int64_t Np = w4_np(N), strips = Np / 4, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool live = id < w4_kb(K) * strips;  // (an even number of strips: a pair of lanes is live or not together)
+  const int64_t kb = live ? id / strips : 0, n0 = live ? (id - kb * strips) * 4 : 0;
+  const bool whole = kb * 32 + 32 <= K && n0 + 4 <= N;
+  u32x4 out[4];
+  uint32_t eall = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t k0 = kb * 32 + j * 8;
+    Vec4<T> v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (whole) {
+        v[i] = *reinterpret_cast<const Vec4<T> *>(W + (k0 + i) * ldw + n0);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[i].v[c] = live && k0 + i < K && n0 + c < N ? W[(k0 + i) * ldw + n0 + c] : T(0.0f);
       }
-  const int eb = bad ? 255 : tile_exp_byte<6, 2, -125>(amax);
-  exps[(kt / 4 * nt + t) * 4 + kt % 4] = (uint8_t)eb;
-  for (int c = 0; c < 8; ++c) {
-    uint32_t w = 0;
+    }
+    uint32_t top = 0;  // the largest magnitude as bits: an infinity or a NaN is above every finite value
+#pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (k0 + i < K && n0 + c < N && !bad) w |= e2m1_code(unscale<6>(to_f32(W[(k0 + i) * ldw + n0 + c]), eb)) << (4 * i);
-    codes[((kt / 4) * Np + n0 + c) * 4 + kt % 4] = w;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, to_f32(v[i].v[c])) & 0x7fffffffu;
+        top = b > top ? b : top;
+      }
+    const uint32_t other = (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xb1, 0xf, 0xf, true);  // the lane next to it
+    const int eb = tile_exp_byte<6, 2, -125>(__builtin_bit_cast(float, other > top ? other : top));
+    eall |= (uint32_t)eb << (8 * j);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w |= e2m1_code(unscale<6>(to_f32(v[i].v[c]), eb)) << (4 * i);
+      out[c][j] = eb == 255 ? 0u : w;
+    }
   }
+  if (!live) return;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) codes[kb * Np + n0 + c] = out[c];
+  if ((id & 1) == 0) exps[kb * (Np / 8) + n0 / 8] = eall;
 }
 
-// value of row k, column n
-__device__ __forceinline__ float w4_value(const uint32_t *codes, const uint8_t *exps, int64_t Np, int64_t k, int64_t n) {
-  const int64_t kb = k / 32;
-  const int j = (int)(k / 8) % 4, i = (int)(k % 8);
-  const uint32_t w = codes[(kb * Np + n) * 4 + j] >> (4 * i);
-  const float s = scale_of(exps[(kb * (Np / 8) + n / 8) * 4 + j]);
-  return bf_lo(w4_pair<0>(w, s));
-}
-
+// The reverse: a thread reads the 64 bytes of its 4 columns and writes 32 rows of 4 elements.
 template <typename T>
-__global__ __launch_bounds__(256) void load_w4_kernel(int64_t K, int64_t N, const uint32_t *__restrict__ codes,
-                                                      const uint8_t *__restrict__ exps, T *__restrict__ out, int64_t ldo) {
-  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, Np = w4_np(N);
-  if (n >= N) return;
-  for (int64_t k = blockIdx.y; k < K; k += gridDim.y) out[k * ldo + n] = from_f32<T>(w4_value(codes, exps, Np, k, n));
+__global__ __launch_bounds__(256) void load_w4_kernel(int64_t K, int64_t N, const u32x4 *__restrict__ codes,
+                                                      const uint32_t *__restrict__ exps, T *__restrict__ out, int64_t ldo) {
+  const int64_t Np = w4_np(N), strips = Np / 4, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= w4_kb(K) * strips) return;
+  const int64_t kb = id / strips, n0 = (id - kb * strips) * 4;
+  u32x4 q[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) q[c] = codes[kb * Np + n0 + c];
+  const uint32_t e = exps[kb * (Np / 8) + n0 / 8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float s = scale_of((e >> (8 * j)) & 255u);
+    u32x4 f[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) f[c] = w4_frag(q[c][j], s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int64_t k = kb * 32 + j * 8 + i;
+      if (k >= K) return;
+      Vec4<T> v;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v.v[c] = from_f32<T>(i & 1 ? bf_hi(f[c][i >> 1]) : bf_lo(f[c][i >> 1]));
+      if (n0 + 4 <= N) {
+        *reinterpret_cast<Vec4<T> *>(out + k * ldo + n0) = v;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (n0 + c < N) out[k * ldo + n0 + c] = v.v[c];
+      }
+    }
+  }
 }
 
 static int check_w4(const char *fn, int dtype, int64_t K, int64_t N, int kn_arg) {
@@ -67,11 +109,11 @@ extern "C" int gpvae_quant_w4(void *stream, int dtype, int64_t K, int64_t N, con
   LB_REQUIRE(ldw >= N, 6, "%s: ldw < N", fn);
   LB_REQUIRE(codes && aligned16(codes), 7, "%s: codes must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(exps && aligned16(exps), 8, "%s: exps must be a 16-byte aligned device pointer", fn);
-  const int64_t tiles = w4_kb(K) * 4 * (w4_np(N) / 8);
-  LB_REQUIRE(cdiv(tiles, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+  const int64_t strips = w4_kb(K) * (w4_np(N) / 4);
+  LB_REQUIRE(cdiv(strips, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
 #define GO(T)                                                                                                         \
-  hipLaunchKernelGGL(quant_w4_kernel<T>, dim3((unsigned)cdiv(tiles, 256)), dim3(256), 0, (hipStream_t)stream, K, N,  \
-                     (const T *)W, ldw, (uint32_t *)codes, (uint8_t *)exps)
+  hipLaunchKernelGGL(quant_w4_kernel<T>, dim3((unsigned)cdiv(strips, 256)), dim3(256), 0, (hipStream_t)stream, K, N,  \
+                     (const T *)W, ldw, (u32x4 *)codes, (uint32_t *)exps)
   LB_BY_DTYPE(dtype, GO);
 #undef GO
   LB_CHECK_LAUNCH(fn);
@@ -86,10 +128,12 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
   LB_REQUIRE(exps && aligned16(exps), 6, "%s: exps must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(out, 7, "%s: out is NULL", fn);
   LB_REQUIRE(ldo >= N, 8, "%s: ldo < N", fn);
-  const dim3 grid((unsigned)cdiv(N, 256), (unsigned)(K < 65535 ? K : 65535));
+  const int64_t strips = w4_kb(K) * (w4_np(N) / 4);
+  LB_REQUIRE(cdiv(strips, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+  const dim3 grid((unsigned)cdiv(strips, 256));
 #define GO(T)                                                                                                     \
-  hipLaunchKernelGGL(load_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, K, N, (const uint32_t *)codes, \
-                     (const uint8_t *)exps, (T *)out, ldo)
+  hipLaunchKernelGGL(load_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, K, N, (const u32x4 *)codes,    \
+                     (const uint32_t *)exps, (T *)out, ldo)
   LB_BY_DTYPE(dtype, GO);
 #undef GO
   LB_CHECK_LAUNCH(fn);
