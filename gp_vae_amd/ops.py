@@ -5,6 +5,7 @@ of caller-visible tensors to libgpvae_hip.so on torch's current HIP stream.  No 
 in torch and nothing falls back to the CPU: a CPU tensor raises.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -696,15 +697,18 @@ def decoder_vjp_static(dec_params, Z, dF, h0, h1, out=None):
 
 
 # ---- dense layers with weights in 4 bits, activation checkpoints in 8 bits (include/gpvae_lowbit.h) -------------
-# The arguments may live on any device: the launch goes to the current stream of THEIR device.
+# The arguments may live on any device: the launch goes to the current stream of THEIR device.  The smallest of these
+# calls last 4 us on the GPU, so the wrappers keep the host's share small: sizes of workspaces are remembered, the stream
+# handle is fetched without a stream object, pointers are passed as plain integers.
 _LB_DT = {torch.float32: LB_F32, torch.bfloat16: LB_BF16, torch.float16: LB_F16}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _lb_dt(what, t):
-    try:
-        return _LB_DT[t.dtype]
-    except KeyError:
+    dt = _LB_DT.get(t.dtype)
+    if dt is None:
         raise GpvaeError("%s: unsupported dtype %s (float32/bfloat16/float16 only)" % (what, t.dtype))
+    return dt
 
 
 def _lb_mat(what, name, t, cols=None, rows=None):
@@ -712,46 +716,58 @@ def _lb_mat(what, name, t, cols=None, rows=None):
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise GpvaeError("%s: %s must be a 2-D tensor" % (what, name))
     _dev(t)
-    if (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows):
+    r, c = t.shape
+    if (cols is not None and c != cols) or (rows is not None and r != rows):
         raise GpvaeError("%s: %s must be [%s, %s]; got %s" % (what, name, "rows" if rows is None else rows,
                                                               "columns" if cols is None else cols, tuple(t.shape)))
-    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-        if t.stride(1) != 1 or t.stride(0) < t.shape[1]:  # torch calls a one-row or one-column view contiguous as it is
-            t = torch.empty_strided(t.shape, (t.shape[1], 1), dtype=t.dtype, device=t.device).copy_(t)
+    s0, s1 = t.stride()
+    if s1 != 1 or s0 < c:  # copied to rows one behind the other (contiguous() keeps the strides of one-row views)
+        t = torch.empty_strided((r, c), (c, 1), dtype=t.dtype, device=t.device).copy_(t)
     return t
 
 
-def _lb_out(what, out, shape, like, src):
+def _lb_out(what, out, rows, cols, like, src):
     if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    if (not isinstance(out, torch.Tensor) or tuple(out.shape) != tuple(shape) or out.dtype != like.dtype
-            or out.device != like.device or out.stride(1) != 1 or out.stride(0) < shape[1]):
+        return like.new_empty((rows, cols))
+    if (not isinstance(out, torch.Tensor) or tuple(out.shape) != (rows, cols) or out.dtype != like.dtype
+            or out.device != like.device or out.stride(1) != 1 or out.stride(0) < cols):
         raise GpvaeError("%s: out must be a %s tensor %s on %s with unit column stride and rows that do not overlap"
-                         % (what, like.dtype, tuple(shape), like.device))
-    if shape[0] and src is not None and out.data_ptr() == src.data_ptr():
+                         % (what, like.dtype, (rows, cols), like.device))
+    if rows and src is not None and out.data_ptr() == src.data_ptr():
         raise GpvaeError("%s: out must not be the input" % what)
     return out
 
 
 def _lb_same(what, dev, *ts):
+    """Every tensor on device number dev."""
     for t in ts:
-        if t is not None and t.device != dev:
-            raise GpvaeError("%s: operands on %s and %s" % (what, dev, t.device))
+        if t is not None and t.get_device() != dev:
+            raise GpvaeError("%s: operands on cuda:%d and %s" % (what, dev, t.device))
 
 
 def _lb_call(what, dev, fn, *args):
-    if dev.index == torch.cuda.current_device():
-        rc = fn(C.c_void_p(torch.cuda.current_stream().cuda_stream), *args)
+    if dev == torch.cuda.current_device():
+        rc = fn(_raw_stream(dev), *args)
     else:
         with torch.cuda.device(dev):
-            rc = fn(C.c_void_p(torch.cuda.current_stream().cuda_stream), *args)
+            rc = fn(_raw_stream(dev), *args)
     if rc:
         check_lowbit(rc, what)
 
 
-def _lb_work(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes > 0 else None
+@functools.lru_cache(maxsize=4096)
+def _lb_work_bytes(name, dt, M, K, N):
+    return getattr(_lib.load_lowbit(), name)(dt, M, K, N)
+
+
+def _lb_work(name, dt, M, K, N, like):
+    """The call's workspace (a tensor, to be kept until the launch) or None."""
+    n = _lb_work_bytes(name, dt, M, K, N)
+    return like.new_empty((n,), dtype=torch.uint8) if n else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 class W4:
@@ -803,55 +819,59 @@ def quant_w4(W):
     if K < 1 or N < 1:
         raise GpvaeError("quant_w4: W must not be empty; got %s" % (tuple(W.shape),))
     kb, np_ = (K + 31) // 32, (N + 31) // 32 * 32
-    codes = torch.empty((kb, np_, 4), dtype=torch.int32, device=W.device)
-    exps = torch.empty((kb, np_ // 8, 4), dtype=torch.uint8, device=W.device)
-    _lb_call("gpvae_quant_w4", W.device, _lib.load_lowbit().gpvae_quant_w4, dt, K, N, _p(W), W.stride(0), _p(codes), _p(exps))
+    codes = W.new_empty((kb, np_, 4), dtype=torch.int32)
+    exps = W.new_empty((kb, np_ // 8, 4), dtype=torch.uint8)
+    _lb_call("gpvae_quant_w4", W.get_device(), _lib.load_lowbit().gpvae_quant_w4, dt, K, N, W.data_ptr(), W.stride(0),
+             codes.data_ptr(), exps.data_ptr())
     return W4(codes, exps, K, N)
 
 
 def load_w4(w4, dtype=torch.float32):
     """The weights [K, N] the codes stand for (exact in float32 and bfloat16)."""
     _dev(w4.codes)
-    out = torch.empty((w4.K, w4.N), dtype=dtype, device=w4.codes.device)
-    _lb_call("gpvae_load_w4", out.device, _lib.load_lowbit().gpvae_load_w4, _lb_dt("load_w4", out), w4.K, w4.N, _p(w4.codes),
-             _p(w4.exps), _p(out), w4.N)
+    out = w4.codes.new_empty((w4.K, w4.N), dtype=dtype)
+    _lb_call("gpvae_load_w4", out.get_device(), _lib.load_lowbit().gpvae_load_w4, _lb_dt("load_w4", out), w4.K, w4.N,
+             w4.codes.data_ptr(), w4.exps.data_ptr(), out.data_ptr(), w4.N)
     return out
 
 
 def dense_w4(X, w4, bias=None, relu=False, out=None):
     """Y = X W + bias [M, N] (relu: max(., 0)) for X [M, K] and weights in 4 bits, for one row or thousands; X float32,
-    bfloat16 or float16, bias [N] and Y of its type, sums in float32."""
-    X = _lb_mat("dense_w4", "X", X, cols=w4.K)
-    dt, dev, M = _lb_dt("dense_w4", X), X.device, X.shape[0]
+    bfloat16 or float16, bias [N] and Y of its type, sums in float32.  out, if given, must not overlap X."""
+    K, N = w4.K, w4.N
+    X = _lb_mat("dense_w4", "X", X, cols=K)
+    dt, dev, M = _lb_dt("dense_w4", X), X.get_device(), X.shape[0]
     if bias is not None:
-        if bias.shape != (w4.N,) or bias.dtype != X.dtype:
-            raise GpvaeError("dense_w4: bias must be a %s tensor [%d]" % (X.dtype, w4.N))
+        if bias.shape != (N,) or bias.dtype != X.dtype:
+            raise GpvaeError("dense_w4: bias must be a %s tensor [%d]" % (X.dtype, N))
         bias = bias.contiguous()
     _lb_same("dense_w4", dev, w4.codes, bias)
-    Y = _lb_out("dense_w4", out, (M, w4.N), X, X)
-    lib = _lib.load_lowbit()
-    work = _lb_work(lib.gpvae_dense_w4_workspace_bytes(dt, M, w4.K, w4.N), dev)
-    _lb_call("gpvae_dense_w4", dev, lib.gpvae_dense_w4, dt, M, w4.K, w4.N, _p(X), X.stride(0), _p(w4.codes), _p(w4.exps),
-             _p(bias), int(bool(relu)), _p(Y), Y.stride(0), _p(work))
+    Y = _lb_out("dense_w4", out, M, N, X, X)
+    work = _lb_work("gpvae_dense_w4_workspace_bytes", dt, M, K, N, X)
+    _lb_call("gpvae_dense_w4", dev, _lib.load_lowbit().gpvae_dense_w4, dt, M, K, N, X.data_ptr(), max(X.stride(0), K),
+             w4.codes.data_ptr(), w4.exps.data_ptr(), _ptr(bias), 1 if relu else 0, Y.data_ptr(), max(Y.stride(0), N), _ptr(work))
     return Y
 
 
 def dense_vjp_w4(dY, w4, act=None, out=None):
     """dX = dY W^T [M, K] for dY [M, N] and weights in 4 bits.  act: the :class:`Q8` checkpoint (relu=True) of the layer's
-    input; dX is then also multiplied by its mask (input > 0), i.e. it is the gradient before the ReLU that made the input."""
-    dY = _lb_mat("dense_vjp_w4", "dY", dY, cols=w4.N)
-    dt, dev, M = _lb_dt("dense_vjp_w4", dY), dY.device, dY.shape[0]
+    input; dX is then also multiplied by its mask (input > 0), i.e. it is the gradient before the ReLU that made the input.
+    out, if given, must not overlap dY."""
+    K, N = w4.K, w4.N
+    dY = _lb_mat("dense_vjp_w4", "dY", dY, cols=N)
+    dt, dev, M = _lb_dt("dense_vjp_w4", dY), dY.get_device(), dY.shape[0]
+    codes = None
     if act is not None:
         if not act.relu:
             raise GpvaeError("dense_vjp_w4: act must be a checkpoint stored with relu=True (its codes carry the mask)")
-        if (act.M, act.K) != (M, w4.K):
-            raise GpvaeError("dense_vjp_w4: act must be a checkpoint of [%d, %d]; got [%d, %d]" % (M, w4.K, act.M, act.K))
-    _lb_same("dense_vjp_w4", dev, w4.codes, None if act is None else act.codes)
-    dX = _lb_out("dense_vjp_w4", out, (M, w4.K), dY, dY)
-    lib = _lib.load_lowbit()
-    work = _lb_work(lib.gpvae_dense_vjp_w4_workspace_bytes(dt, M, w4.K, w4.N), dev)
-    _lb_call("gpvae_dense_vjp_w4", dev, lib.gpvae_dense_vjp_w4, dt, M, w4.K, w4.N, _p(dY), dY.stride(0), _p(w4.codes),
-             _p(w4.exps), _p(None if act is None else act.codes), _p(dX), dX.stride(0), _p(work))
+        if act.M != M or act.K != K:
+            raise GpvaeError("dense_vjp_w4: act must be a checkpoint of [%d, %d]; got [%d, %d]" % (M, K, act.M, act.K))
+        codes = act.codes
+    _lb_same("dense_vjp_w4", dev, w4.codes, codes)
+    dX = _lb_out("dense_vjp_w4", out, M, K, dY, dY)
+    work = _lb_work("gpvae_dense_vjp_w4_workspace_bytes", dt, M, K, N, dY)
+    _lb_call("gpvae_dense_vjp_w4", dev, _lib.load_lowbit().gpvae_dense_vjp_w4, dt, M, K, N, dY.data_ptr(), max(dY.stride(0), N),
+             w4.codes.data_ptr(), w4.exps.data_ptr(), _ptr(codes), dX.data_ptr(), max(dX.stride(0), K), _ptr(work))
     return dX
 
 
@@ -861,22 +881,26 @@ def store_q8(X, relu=False, out=None):
     A tile with an infinity or a NaN reads as NaN; its ReLU mask stays that of the values (NaN passes)."""
     src = X
     X = _lb_mat("store_q8", "X", X)
-    dt, dev = _lb_dt("store_q8", X), X.device
+    dt, dev = _lb_dt("store_q8", X), X.get_device()
     M, K = X.shape
     if K < 1:
         raise GpvaeError("store_q8: X must have at least one column; got %s" % (tuple(X.shape),))
-    if out is not None and not relu:
-        raise GpvaeError("store_q8: out is the ReLU's output (relu=True)")
-    if out is not None and X is not src and out is src:
-        raise GpvaeError("store_q8: in place needs unit column stride and rows that do not overlap")
-    Y = _lb_out("store_q8", out, (M, K), X, None) if relu else None
-    if Y is not None and M and Y.data_ptr() == X.data_ptr() and M > 1 and Y.stride(0) != X.stride(0):
-        raise GpvaeError("store_q8: in place needs equal strides")
+    Y = None
+    if out is not None:
+        if not relu:
+            raise GpvaeError("store_q8: out is the ReLU's output (relu=True)")
+        if X is not src and out is src:
+            raise GpvaeError("store_q8: in place needs unit column stride and rows that do not overlap")
+    if relu:
+        Y = _lb_out("store_q8", out, M, K, X, None)
+        if M > 1 and Y.data_ptr() == X.data_ptr() and Y.stride(0) != X.stride(0):
+            raise GpvaeError("store_q8: in place needs equal strides")
     mb, kp = (M + 7) // 8, (K + 31) // 32 * 32
-    codes = torch.empty((mb, kp, 8), dtype=torch.uint8, device=dev)
-    exps = torch.empty((mb, kp // 8), dtype=torch.uint8, device=dev)
-    _lb_call("gpvae_store_q8", dev, _lib.load_lowbit().gpvae_store_q8, dt, M, K, _p(X), X.stride(0), int(bool(relu)), _p(Y),
-             Y.stride(0) if relu else 0, _p(codes), _p(exps))
+    codes = X.new_empty((mb, kp, 8), dtype=torch.uint8)
+    exps = X.new_empty((mb, kp // 8), dtype=torch.uint8)
+    ldx = max(X.stride(0), K)
+    _lb_call("gpvae_store_q8", dev, _lib.load_lowbit().gpvae_store_q8, dt, M, K, X.data_ptr(), ldx, 1 if relu else 0, _ptr(Y),
+             0 if Y is None else ldx if M == 1 else Y.stride(0), codes.data_ptr(), exps.data_ptr())
     q8 = Q8(codes, exps, M, K, relu)
     return (Y, q8) if relu else q8
 
@@ -884,9 +908,9 @@ def store_q8(X, relu=False, out=None):
 def load_q8(q8, dtype=torch.float32):
     """The values [M, K] a checkpoint stands for (exact in float32 and bfloat16)."""
     _dev(q8.codes)
-    out = torch.empty((q8.M, q8.K), dtype=dtype, device=q8.codes.device)
-    _lb_call("gpvae_load_q8", out.device, _lib.load_lowbit().gpvae_load_q8, _lb_dt("load_q8", out), q8.M, q8.K, int(q8.relu),
-             _p(q8.codes), _p(q8.exps), _p(out), q8.K)
+    out = q8.codes.new_empty((q8.M, q8.K), dtype=dtype)
+    _lb_call("gpvae_load_q8", out.get_device(), _lib.load_lowbit().gpvae_load_q8, _lb_dt("load_q8", out), q8.M, q8.K,
+             1 if q8.relu else 0, q8.codes.data_ptr(), q8.exps.data_ptr(), out.data_ptr(), q8.K)
     return out
 
 
@@ -894,23 +918,24 @@ def dense_grads_q8(q8, dY, out=None):
     """(dW [K, N], db [N]) float32 of a dense layer y = x W + b from the 8-bit checkpoint of its input x [M, K] and
     dY [M, N] (float32, bfloat16 or float16): dW = x~^T dY, db = sum of dY's rows.  out: optional pair (dW, db) of float32
     tensors to write to (db may be None: not wanted)."""
-    dY = _lb_mat("dense_grads_q8", "dY", dY, rows=q8.M)
-    dt, dev, N = _lb_dt("dense_grads_q8", dY), dY.device, dY.shape[1]
+    M, K = q8.M, q8.K
+    dY = _lb_mat("dense_grads_q8", "dY", dY, rows=M)
+    dt, dev, N = _lb_dt("dense_grads_q8", dY), dY.get_device(), dY.shape[1]
     if N < 1:
         raise GpvaeError("dense_grads_q8: dY must have at least one column")
     _lb_same("dense_grads_q8", dev, q8.codes)
     if out is None:
-        dW = torch.empty((q8.K, N), dtype=torch.float32, device=dev)
-        db = torch.empty((N,), dtype=torch.float32, device=dev)
+        dW, db = dY.new_empty((K, N), dtype=torch.float32), dY.new_empty((N,), dtype=torch.float32)
     else:
         dW, db = out
-        if (tuple(dW.shape) != (q8.K, N) or dW.dtype != torch.float32 or dW.device != dev or dW.stride(1) != 1
+        if (tuple(dW.shape) != (K, N) or dW.dtype != torch.float32 or dW.get_device() != dev or dW.stride(1) != 1
                 or dW.stride(0) < N):
-            raise GpvaeError("dense_grads_q8: dW must be float32 [%d, %d] on %s, unit column stride" % (q8.K, N, dev))
-        if db is not None and (tuple(db.shape) != (N,) or db.dtype != torch.float32 or db.device != dev or not db.is_contiguous()):
-            raise GpvaeError("dense_grads_q8: db must be contiguous float32 [%d] on %s" % (N, dev))
-    lib = _lib.load_lowbit()
-    work = _lb_work(lib.gpvae_dense_grads_q8_workspace_bytes(dt, q8.M, q8.K, N), dev)
-    _lb_call("gpvae_dense_grads_q8", dev, lib.gpvae_dense_grads_q8, dt, q8.M, q8.K, N, int(q8.relu), _p(q8.codes), _p(q8.exps),
-             _p(dY), dY.stride(0), _p(dW), dW.stride(0), _p(db), _p(work))
+            raise GpvaeError("dense_grads_q8: dW must be float32 [%d, %d] on %s, unit column stride" % (K, N, dY.device))
+        if db is not None and (tuple(db.shape) != (N,) or db.dtype != torch.float32 or db.get_device() != dev
+                               or not db.is_contiguous()):
+            raise GpvaeError("dense_grads_q8: db must be contiguous float32 [%d] on %s" % (N, dY.device))
+    work = _lb_work("gpvae_dense_grads_q8_workspace_bytes", dt, M, K, N, dY)
+    _lb_call("gpvae_dense_grads_q8", dev, _lib.load_lowbit().gpvae_dense_grads_q8, dt, M, K, N, 1 if q8.relu else 0,
+             q8.codes.data_ptr(), q8.exps.data_ptr(), dY.data_ptr(), max(dY.stride(0), N), dW.data_ptr(), dW.stride(0), _ptr(db),
+             _ptr(work))
     return dW, db
