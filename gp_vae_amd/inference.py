@@ -353,16 +353,28 @@ class GPInference(Inference):
 
 
 class VAEInference(Inference):
-    """MCMC with the trained decoder as prior (inference.py:208-254)."""
+    """MCMC with the trained decoder as prior (inference.py:208-254).
 
-    def __init__(self, decoder, decoder_params, z_dim, *args, **kwargs):
+    weights="w4" (float32 only): the decoder's weight matrices are kept in 4 bits (ops.quant_decoder_w4) and every use of
+    the decoder — predict, the potential and its gradient — is that decoder's, the ReLU masks of the gradient read from the
+    forward pass's 8-bit checkpoints.  For wide decoders, whose weights are what an evaluation reads; the chains
+    then run in lock step over the composed potential, not in the fused kernels of the small ones."""
+
+    def __init__(self, decoder, decoder_params, z_dim, *args, weights="float", **kwargs):
         super().__init__(*args, **kwargs)
+        if weights not in ("float", "w4"):
+            raise ValueError("weights must be 'float' or 'w4'")
+        if weights == "w4" and self.dtype != torch.float32:
+            raise GpvaeError("VAEInference: weights='w4' is a float32 path; got %s" % self.dtype)
         self.decoder = decoder
         self.decoder_params = decoder_params
         self.z_dim = z_dim
         (V1, _), _, (V2, _), _, (V3, _) = decoder_params
         self.h1, self.h0, self.n_out = V1.shape[1], V2.shape[1], V3.shape[1]
         self.dec_flat = decoder_flat_from_list(decoder_params, self.dtype)
+        self.dec_w4 = None
+        if weights == "w4":
+            self.dec_w4 = ops.quant_decoder_w4(self.dec_flat, self.n_out, self.h0, self.h1, self.z_dim)
         ops.check_index(self.obs_idx, self.n_out, "obs_idx (decoder outputs)")
 
     def regression(self, y=None, obs_idx=None, rng_key=None, num_samples=None, posterior_samples=None):
@@ -392,7 +404,7 @@ class VAEInference(Inference):
 
         y_obs = y_obs.contiguous()
         idx = idx.contiguous()
-        fused = ops.vae_potential_supported(dt, self.h0, self.h1, zd, idx.numel())
+        fused = self.dec_w4 is None and ops.vae_potential_supported(dt, self.h0, self.h1, zd, idx.numel())
 
         def fn(q):
             if fused:  # one launch per evaluation (gpvae_vae_potential)
@@ -447,8 +459,10 @@ class VAEInference(Inference):
 
     def predict(self, z):
         """f = decoder(decoder_params, z) for a batch of latent vectors [chains, z_dim]."""
-        return ops.decoder_fwd(self.dec_flat, _as_device(z, self.dtype).reshape(-1, self.z_dim),
-                               self.n_out, self.h0, self.h1)
+        z = _as_device(z, self.dtype).reshape(-1, self.z_dim)
+        if self.dec_w4 is not None:
+            return ops.decoder_fwd_w4(self.dec_w4, z)
+        return ops.decoder_fwd(self.dec_flat, z, self.n_out, self.h0, self.h1)
 
     def potential_and_grad(self, z, log_sigma):
         """Potential energy of VAEInference.regression (inference.py:243-254) in NumPyro's
@@ -459,7 +473,7 @@ class VAEInference(Inference):
         Returns (U [chains], dU/dz [chains, z_dim], dU/dlog_sigma [chains]).  The decoder forward and
         its vector-Jacobian product are the HIP kernels; the O(chains * n_obs) tail is glue."""
         zz = _as_device(z, self.dtype).reshape(-1, self.z_dim)
-        if ops.vae_potential_supported(self.dtype, self.h0, self.h1, self.z_dim, self.obs_idx.numel()):
+        if self.dec_w4 is None and ops.vae_potential_supported(self.dtype, self.h0, self.h1, self.z_dim, self.obs_idx.numel()):
             q = torch.cat([zz, _as_device(log_sigma, self.dtype).reshape(-1, 1)], 1)
             U, dU = ops.vae_potential(self.dec_flat, q, self.y[self.obs_idx].contiguous(), self.obs_idx.contiguous(),
                                       self.n_out, self.h0, self.h1, checked=True)  # obs_idx was checked in __init__
@@ -470,7 +484,11 @@ class VAEInference(Inference):
         z = _as_device(z, self.dtype).reshape(-1, self.z_dim).contiguous()
         u = _as_device(log_sigma, self.dtype).reshape(-1)
         sigma = torch.exp(u)
-        f = ops.decoder_fwd(self.dec_flat, z, self.n_out, self.h0, self.h1)
+        acts = None
+        if self.dec_w4 is not None:
+            f, acts = ops.decoder_fwd_w4(self.dec_w4, z, keep=True)
+        else:
+            f = ops.decoder_fwd(self.dec_flat, z, self.n_out, self.h0, self.h1)
         r = f[:, obs_idx] - y_obs[None, :]
         n_obs = obs_idx.numel()
         s0 = 0.1
@@ -482,6 +500,7 @@ class VAEInference(Inference):
         U = -(log_lik + log_pz + log_ps)
         dF = torch.zeros_like(f)
         dF.index_add_(1, obs_idx, r / (sigma ** 2)[:, None])  # repeats in obs_idx accumulate
-        dz = z + ops.decoder_vjp(self.dec_flat, z, dF, self.h0, self.h1)
+        dz = z + (ops.decoder_vjp(self.dec_flat, z, dF, self.h0, self.h1) if acts is None
+                  else ops.decoder_vjp_w4(self.dec_w4, acts, dF))
         du = (sigma / s0) ** 2 - 1.0 + n_obs - sq / sigma ** 2
         return U, dz, du

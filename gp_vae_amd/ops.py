@@ -939,3 +939,78 @@ def dense_grads_q8(q8, dY, out=None):
              q8.codes.data_ptr(), q8.exps.data_ptr(), dY.data_ptr(), max(dY.stride(0), N), dW.data_ptr(), dW.stride(0), _ptr(db),
              _ptr(work))
     return dW, db
+
+
+# ---- the VAE's decoder in 4 bits: the layers above composed like decoder_fwd / decoder_vjp ---------------------------
+class DecoderW4:
+    """The decoder (z -> h1 -> h0 -> n, ReLU between; decoder_fwd's layers) with its three weight matrices in 4 bits and its
+    biases as they are.  Made by quant_decoder_w4."""
+
+    __slots__ = ("layers", "biases", "z", "h1", "h0", "n", "dtype")
+
+    def __init__(self, layers, biases):
+        self.layers, self.biases = tuple(layers), tuple(biases)
+        self.z, self.h1, self.h0, self.n = self.layers[0].K, self.layers[0].N, self.layers[1].N, self.layers[2].N
+        if self.layers[1].K != self.h1 or self.layers[2].K != self.h0:
+            raise GpvaeError("DecoderW4: layer shapes do not chain")
+        self.dtype = self.biases[0].dtype
+        for w, b in zip(self.layers, self.biases):
+            if tuple(b.shape) != (w.N,) or b.dtype != self.dtype:
+                raise GpvaeError("DecoderW4: biases must be %s vectors of the layers' widths" % self.dtype)
+
+
+def quant_decoder_w4(dec_params, n, h0, h1, z):
+    """The flat decoder parameters V1 c1 V2 c2 V3 c3 (decoder_fwd's; float32, bfloat16 or float16) as a :class:`DecoderW4`."""
+    _dev(dec_params)
+    _lb_dt("quant_decoder_w4", dec_params)
+    want = z * h1 + h1 + h1 * h0 + h0 + h0 * n + n
+    if dec_params.dim() != 1 or dec_params.numel() != want or not dec_params.is_contiguous():
+        raise GpvaeError("quant_decoder_w4: dec_params must be a contiguous vector of %d elements for (n, h0, h1, z)" % want)
+    layers, biases, o = [], [], 0
+    for k, w in ((z, h1), (h1, h0), (h0, n)):
+        layers.append(quant_w4(dec_params[o:o + k * w].view(k, w)))
+        o += k * w
+        biases.append(dec_params[o:o + w].clone())
+        o += w
+    return DecoderW4(layers, biases)
+
+
+def decoder_fwd_w4(dec, Z, keep=False):
+    """F [chains, n] = decoder(Z) with weights in 4 bits, Z [chains, z] of dec.dtype.  keep=True: (F, acts), acts the 8-bit
+    checkpoints (Z, D1, D2) of the three layers' inputs for decoder_vjp_w4."""
+    Z = _lb_mat("decoder_fwd_w4", "Z", Z, cols=dec.z)
+    if Z.dtype != dec.dtype:
+        raise GpvaeError("decoder_fwd_w4: Z must be %s" % dec.dtype)
+    (W1, W2, W3), (c1, c2, c3) = dec.layers, dec.biases
+    if not keep:
+        return dense_w4(dense_w4(dense_w4(Z, W1, c1, relu=True), W2, c2, relu=True), W3, c3)
+    D1 = dense_w4(Z, W1, c1)
+    _, a1 = store_q8(D1, relu=True, out=D1)
+    D2 = dense_w4(D1, W2, c2)
+    _, a2 = store_q8(D2, relu=True, out=D2)
+    return dense_w4(D2, W3, c3), (store_q8(Z), a1, a2)
+
+
+def decoder_vjp_w4(dec, acts, dF, grads=False):
+    """dZ [chains, z] = dF [chains, n] times the Jacobian of decoder_fwd_w4 at the Z that left `acts`: the ReLU masks come from
+    the checkpoints (exact), nothing is recomputed.  grads=True: (dZ, dparams), dparams the float32 gradient of the
+    parameters, flat like dec_params (V1 c1 V2 c2 V3 c3; that of the weights is the one at their 4-bit values, with the
+    layers' inputs in 8 bits)."""
+    a0, a1, a2 = acts
+    (W1, W2, W3) = dec.layers
+    dF = _lb_mat("decoder_vjp_w4", "dF", dF, cols=dec.n, rows=a0.M)
+    if dF.dtype != dec.dtype:
+        raise GpvaeError("decoder_vjp_w4: dF must be %s" % dec.dtype)
+    d2 = dense_vjp_w4(dF, W3, a2)
+    d1 = dense_vjp_w4(d2, W2, a1)
+    dZ = dense_vjp_w4(d1, W1)
+    if not grads:
+        return dZ
+    flat = dF.new_empty((dec.z * dec.h1 + dec.h1 + dec.h1 * dec.h0 + dec.h0 + dec.h0 * dec.n + dec.n,), dtype=torch.float32)
+    o = 0
+    for a, d, w in ((a0, d1, W1), (a1, d2, W2), (a2, dF, W3)):
+        dW = flat[o:o + w.K * w.N].view(w.K, w.N)
+        o += w.K * w.N
+        dense_grads_q8(a, d, out=(dW, flat[o:o + w.N]))
+        o += w.N
+    return dZ, flat
