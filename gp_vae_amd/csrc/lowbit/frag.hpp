@@ -21,9 +21,10 @@ __device__ __forceinline__ int64_t xcd_chunk(int64_t id, int64_t n) {
 }
 
 // ---- w4 -----------------------------------------------------------------------------------------------------------------
-// 8 codes -> 8 bfloat16 values; byte J of the tile-exponent word e is their exponent
+// 8 codes -> 8 bfloat16 values; byte J of the tile-exponent word e is their exponent.  The conversion uses the scale's exponent
+// bits alone (checked over all exponents with random sign and mantissa bits): the neighbouring bytes need no masking.
 template <int J> __device__ __forceinline__ float w4_scale(uint32_t e) {
-  return __builtin_bit_cast(float, (J == 0 ? e << 23 : J == 1 ? e << 15 : J == 2 ? e << 7 : e >> 1) & 0x7f800000u);
+  return __builtin_bit_cast(float, J == 0 ? e << 23 : J == 1 ? e << 15 : J == 2 ? e << 7 : e >> 1);
 }
 __device__ __forceinline__ u32x4 w4_frag(uint32_t w, float scale) {
   return u32x4{w4_pair<0>(w, scale), w4_pair<1>(w, scale), w4_pair<2>(w, scale), w4_pair<3>(w, scale)};
@@ -52,7 +53,7 @@ struct Tr8 {
     x = __builtin_amdgcn_perm(p, x, sel2);
     p = (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true);            // quad_perm [1,0,3,2]
     p = __builtin_amdgcn_alignbit(p, p, rot);
-    return (own & x) | (~own & p);
+    return p ^ (own & (x ^ p));  // own ? x : p, bit by bit
   }
 };
 
@@ -100,7 +101,7 @@ template <> struct Split<__bf16> {
 // four elements at any element-aligned address: one vector load (unaligned access is on)
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Vec4 { T v[4]; };
 
-// v[0..3] = row[k .. k + 3], zero from L on
+// v[0..3] = row[k .. k + 3], zero from L on (k may lie past L)
 template <typename T> __device__ __forceinline__ Vec4<T> load4(const T *row, int64_t k, int64_t L) {
   Vec4<T> v;
   if (k + 4 <= L) {
@@ -140,6 +141,20 @@ template <typename T, bool VJP> struct Epilogue {
   }
 };
 
+// p[0] + p[stride] + ... (n terms) in order, eight loads in flight at a time
+__device__ __forceinline__ float sum_parts(const float *p, int64_t stride, int n) {
+  float v = 0.0f;
+  for (int s = 0; s < n; s += 8) {
+    float t[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) t[u] = p[(s + u < n ? s + u : n - 1) * stride];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (s + u < n) v += t[u];
+  }
+  return v;
+}
+
 // the sum of the partial outputs [splits][M][O] in order, and the epilogue
 template <typename T, bool VJP>
 __global__ __launch_bounds__(256) void split_sum_kernel(int64_t M, int64_t O, int splits, const float *__restrict__ part,
@@ -149,9 +164,7 @@ __global__ __launch_bounds__(256) void split_sum_kernel(int64_t M, int64_t O, in
   const int64_t m = i / O, o = i - m * O;
   const float b = ep.bias_at(o);
   const uint32_t mask = ep.mask_at(m, o);
-  float v = 0.0f;
-  for (int s = 0; s < splits; ++s) v += part[s * M * O + i];
-  ep.store(m, o, v, b, mask);
+  ep.store(m, o, sum_parts(part + i, M * O, splits), b, mask);
 }
 
 }  // namespace gpvae_lb

@@ -198,8 +198,7 @@ static __global__ __launch_bounds__(256) void grads_sum_kernel(int64_t K, int64_
                                                                float *__restrict__ dW, int64_t lddw, float *__restrict__ db) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (K + 1) * N;
   if (i >= (db ? all : K * N)) return;
-  float v = 0.0f;
-  for (int s = 0; s < splits; ++s) v += part[s * all + i];
+  const float v = sum_parts(part + i, all, splits);
   const int64_t k = i / N, n = i - k * N;
   if (k < K) dW[k * lddw + n] = v;
   else db[n] = v;

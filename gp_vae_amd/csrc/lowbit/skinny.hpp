@@ -49,9 +49,9 @@ static inline SkinnyPlan skinny_plan(int64_t rows, int64_t L, int64_t O) {
 
 template <typename T, bool VJP, int RT>
 __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_t L, int64_t O, const T *__restrict__ X,
-                                                               int64_t ldx, const u32x4 *__restrict__ codes,
-                                                               const uint32_t *__restrict__ exps, int64_t Np, int64_t kbs,
-                                                               int wk_n, int steps, int chunk, float *__restrict__ part,
+                                                               int64_t ldx, const char *__restrict__ codes,
+                                                               const char *__restrict__ exps, int64_t Np, int64_t kbs,
+                                                               int wk_n, int steps, int chunk, uint32_t magic, float *__restrict__ part,
                                                                Epilogue<T, VJP> ep) {
   constexpr int P = Split<T>::P;
   __shared__ __align__(16) unsigned char lds[skinny_lds(RT)];
@@ -70,24 +70,32 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
 
   u32x2 cw[4];  // codes of one step: 16 bytes for each of two columns, or 8 bytes for each of four
   uint32_t ce[VJP ? 4 : 2];
-  auto fetch = [&](int64_t s) {
-    // past the ends the last codes are read again: their outputs are unused, or they meet the image's zeros
+  const uint32_t coff = VJP ? (c * 8 + lab) * 16 + half * 8 : (uint32_t)((c * Np + l16) * 16);
+  const uint32_t eoff = VJP ? c * 4 : (uint32_t)(c * (Np / 2) + (l16 >> 3) * 4);
+  // last step with codes, and how many blocks of 32 rows (quarters of 32 columns) it has
+  const int s_last = (int)((VJP ? Np - 1 : (kbs - 1) * 32) / 128);
+  const int part_last = VJP ? (int)(Np - (int64_t)s_last * 128) / 32 - 1 : (int)(kbs - 1 - 4 * (int64_t)s_last);
+  const char *const cbase = codes + (VJP ? o0 / 32 * Np : o0) * 16, *const ebase = exps + (VJP ? o0 / 32 * Np : o0) / 2;
+  const uint32_t cstep = VJP ? 2048u : (uint32_t)(Np * 64), estep = VJP ? 64u : (uint32_t)(Np * 2);
+  auto fetch = [&](int s) __attribute__((always_inline)) {
+    const int sc = s < s_last ? s : s_last, last = s < s_last ? 3 : part_last;
+    const char *const cb = cbase + (uint64_t)(uint32_t)sc * cstep, *const eb = ebase + (uint64_t)(uint32_t)sc * estep;
     if (!VJP) {
-      const int64_t kb = 4 * s + c < kbs ? 4 * s + c : kbs - 1;
+      const uint32_t back = c > last ? (uint32_t)(c - last) : 0u;  // blocks past the last: that one
+      const uint32_t co = coff - back * (cstep / 4), eo = eoff - back * (estep / 4);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const int64_t n = o0 + t * 16 + l16;
-        const u32x4 q = codes[kb * Np + n];
+        const u32x4 q = *reinterpret_cast<const u32x4 *>(cb + t * 256 + co);
         cw[2 * t] = u32x2{q.x, q.y};
         cw[2 * t + 1] = u32x2{q.z, q.w};
-        ce[t] = exps[kb * (Np / 8) + n / 8];
+        ce[t] = *reinterpret_cast<const uint32_t *>(eb + t * 8 + eo);
       }
     } else {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int64_t n0 = s * 128 + t * 32 < Np ? s * 128 + t * 32 : Np - 32;
-        cw[t] = reinterpret_cast<const u32x2 *>(codes)[(o0 / 32 * Np + n0 + c * 8 + lab) * 2 + half];
-        ce[t] = exps[o0 / 32 * (Np / 8) + n0 / 8 + c];
+        const uint32_t back = t > last ? (uint32_t)(t - last) : 0u;  // quarters past the last: that one
+        cw[t] = *reinterpret_cast<const u32x2 *>(cb + (coff + (t - back) * 512));  // t >= back: no wrap before the addition
+        ce[t] = *reinterpret_cast<const uint32_t *>(eb + (eoff + (t - back) * 16));
       }
     }
   };
@@ -98,7 +106,7 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
 #pragma unroll
     for (int t = 0; t < 2; ++t) acc[r][t] = f32x4_t{0, 0, 0, 0};
 
-  fetch(s_lo + wk);
+  fetch((int)s_lo + wk);
   int a_off[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
@@ -109,16 +117,26 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
   for (int64_t s0 = s_lo; s0 < s_hi; s0 += chunk_steps) {
     if (s0 != s_lo) __syncthreads();
     {  // the image of reduction indices [128 s0, 128 s0 + chunk): 4 at a time, zeros past L
-      const int q = chunk / 4;
-      for (int i = tid; i < (int)M * q; i += 64 * SK_WAVES) {
-        const int m = i / q, k4 = i - m * q;
-        const Vec4<T> v = load4(X + m * ldx, s0 * 128 + k4 * 4, L);
+      const int q = chunk / 4;  // magic = ceil(2^32 / q): exact quotients, i < 2^32 / q
+      auto put = [&](int m, int k4, const Vec4<T> &v) __attribute__((always_inline)) {
         uint32_t a[P], b[P];
         Split<T>::two(v.v[0], v.v[1], a);
         Split<T>::two(v.v[2], v.v[3], b);
 #pragma unroll
         for (int p = 0; p < P; ++p)
           *reinterpret_cast<u32x2 *>(lds + (p * (int)M + m) * stride + k4 * 8) = u32x2{a[p], b[p]};
+      };
+      const T *const x0 = X + s0 * 128;
+      if (s0 * 128 + chunk <= L) {
+        for (int i = tid; i < (int)M * q; i += 64 * SK_WAVES) {
+          const int m = (int)__umulhi((uint32_t)i, magic), k4 = i - m * q;
+          put(m, k4, *reinterpret_cast<const Vec4<T> *>(x0 + m * ldx + k4 * 4));
+        }
+      } else {
+        for (int i = tid; i < (int)M * q; i += 64 * SK_WAVES) {
+          const int m = (int)__umulhi((uint32_t)i, magic), k4 = i - m * q;
+          put(m, k4, load4(x0 + m * ldx, k4 * 4, L - s0 * 128));
+        }
       }
     }
     __syncthreads();
@@ -131,7 +149,7 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
       for (int t = 0; t < 4; ++t) w[t] = cw[t];
 #pragma unroll
       for (int t = 0; t < (VJP ? 4 : 2); ++t) e[t] = ce[t];
-      fetch(s + wk_n);
+      fetch((int)s + wk_n);
       const unsigned char *img = lds + i * 256;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -204,7 +222,7 @@ static void launch_skinny(hipStream_t st, const SkinnyPlan &p, int64_t M, int64_
   const dim3 grid((unsigned)p.gx, (unsigned)p.splits);
 #define GO(RT)                                                                                                            \
   hipLaunchKernelGGL((skinny_kernel<T, VJP, RT>), grid, dim3(64 * SK_WAVES), 0, st, M, L, O, X, ldx,                    \
-                     (const u32x4 *)codes, (const uint32_t *)exps, Np, kbs, p.wk, p.steps, p.chunk, part, ep)
+                     (const char *)codes, (const char *)exps, Np, kbs, p.wk, p.steps, p.chunk, (uint32_t)cdiv(int64_t(1) << 32, p.chunk / 4), part, ep)
   if (p.rt == 1) GO(1);
   else if (p.rt == 2) GO(2);
   else if (p.rt == 3) GO(3);

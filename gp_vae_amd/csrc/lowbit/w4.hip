@@ -91,9 +91,9 @@ __global__ __launch_bounds__(256) void load_w4_kernel(int64_t K, int64_t N, cons
 
 static int check_w4(const char *fn, int dtype, int64_t K, int64_t N, int kn_arg) {
   LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
-  // N: two rows of code words lie within a 32-bit offset
+  // N: four rows of code words lie within a 32-bit offset
   LB_REQUIRE(K >= 1 && K <= (1 << 30), kn_arg, "%s: K must lie in [1, 2^30] (got %lld)", fn, (long long)K);
-  LB_REQUIRE(N >= 1 && N <= (1 << 26), kn_arg + 1, "%s: N must lie in [1, 2^26] (got %lld)", fn, (long long)N);
+  LB_REQUIRE(N >= 1 && N <= (1 << 25), kn_arg + 1, "%s: N must lie in [1, 2^25] (got %lld)", fn, (long long)N);
   return 0;
 }
 
