@@ -21,19 +21,26 @@ struct SkinnyPlan {
   int splits;    // workgroups along the reduction
   int steps;     // steps of 128 reduction indices of one split (a multiple of chunk / 128 unless it is the only chunk)
   int64_t gx;    // workgroups along the outputs
+  int groups, mg;  // groups of rows (each reads all codes) and rows of one
 };
 static constexpr int skinny_lds(int rt) { return rt <= 1 ? 40 << 10 : rt == 2 ? 56 << 10 : 72 << 10; }
 
-static inline SkinnyPlan skinny_plan(int64_t rows, int64_t L, int64_t O) {
+// P pieces of M rows, L reduction indices, O outputs
+static inline SkinnyPlan skinny_plan(int P, int64_t M, int64_t L, int64_t O) {
   SkinnyPlan p;
+  p.groups = (int)cdiv(M, SK_MAXROWS / P);
+  p.mg = (int)cdiv(M, p.groups);
+  const int rows = P * p.mg;
   p.rt = (int)cdiv(rows, 16);
   const int64_t steps = cdiv(L, 128), tiles = cdiv(O, 32);
   const int room = (int)((skinny_lds(p.rt) / rows - 16) / 256);  // steps whose image fits
   p.wk = 1;
   while (p.wk < SK_WAVES && 2 * p.wk <= steps && 2 * p.wk <= room && tiles * p.wk < 2048) p.wk *= 2;
   p.gx = cdiv(tiles, SK_WAVES / p.wk);
-  int64_t s = p.gx < 256 ? cdiv(512, p.gx) : 1;
-  const int64_t most = steps / (4 * p.wk);  // a split keeps four steps for each of its waves
+  int64_t s = p.gx * p.groups < 256 ? cdiv(512, p.gx * p.groups) : 1;
+  // a split costs a second launch (3 us): worth it down to four steps of each wave for one operand tile, to one for three or
+  // four, whose steps take longer (16 x 1024 x 4096 transposed: 15.0 us at four, 11.2 at two, 9.5 at one; 1 x 4096 x 1024: 5.5, 6.7, 6.3)
+  const int64_t most = steps / ((p.rt == 1 ? 4 : p.rt == 2 ? 2 : 1) * p.wk);
   if (s > most) s = most;
   if (s < 1) s = 1;
   if (s > 64) s = 64;
@@ -48,7 +55,7 @@ static inline SkinnyPlan skinny_plan(int64_t rows, int64_t L, int64_t O) {
 }
 
 template <typename T, bool VJP, int RT>
-__global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_t L, int64_t O, const T *__restrict__ X,
+__global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M_all, int mg, int64_t L, int64_t O, const T *__restrict__ X,
                                                                int64_t ldx, const char *__restrict__ codes,
                                                                const char *__restrict__ exps, int64_t Np, int64_t kbs,
                                                                int wk_n, int steps, int chunk, uint32_t magic, float *__restrict__ part,
@@ -58,9 +65,12 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave & (wk_n - 1), wn = wave / wk_n;
   const int c = lane >> 4, l16 = lane & 15;
+  const int64_t m_lo = (int64_t)blockIdx.z * mg;  // this group of rows
+  const int M = m_lo + mg <= M_all ? mg : (int)(M_all - m_lo);
+  X += m_lo * ldx;
   const int64_t tile = (int64_t)blockIdx.x * (SK_WAVES / wk_n) + wn;  // 32 outputs
   const int64_t o0 = (tile * 32 < O ? tile : (O - 1) / 32) * 32;           // a wave past the last tile repeats it, unused
-  const int rows = P * (int)M;
+  const int rows = P * M;
   const int stride = chunk * 2 + 16;  // bytes of an image row: 16 more spread the rows over the banks
   const int64_t s_all = cdiv(L, 128), s_lo = (int64_t)blockIdx.y * steps;
   const int64_t s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
@@ -124,16 +134,16 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
         Split<T>::two(v.v[2], v.v[3], b);
 #pragma unroll
         for (int p = 0; p < P; ++p)
-          *reinterpret_cast<u32x2 *>(lds + (p * (int)M + m) * stride + k4 * 8) = u32x2{a[p], b[p]};
+          *reinterpret_cast<u32x2 *>(lds + (p * M + m) * stride + k4 * 8) = u32x2{a[p], b[p]};
       };
       const T *const x0 = X + s0 * 128;
       if (s0 * 128 + chunk <= L) {
-        for (int i = tid; i < (int)M * q; i += 64 * SK_WAVES) {
+        for (int i = tid; i < M * q; i += 64 * SK_WAVES) {
           const int m = (int)__umulhi((uint32_t)i, magic), k4 = i - m * q;
           put(m, k4, *reinterpret_cast<const Vec4<T> *>(x0 + m * ldx + k4 * 4));
         }
       } else {
-        for (int i = tid; i < (int)M * q; i += 64 * SK_WAVES) {
+        for (int i = tid; i < M * q; i += 64 * SK_WAVES) {
           const int m = (int)__umulhi((uint32_t)i, magic), k4 = i - m * q;
           put(m, k4, load4(x0 + m * ldx, k4 * 4, L - s0 * 128));
         }
@@ -193,24 +203,24 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M, int64_
   if (o >= O) return;
   const bool whole = gridDim.y == 1;
   const float b = whole ? ep.bias_at(o) : 0.0f;
-  for (int m0 = tid / outs; m0 < (int)M; m0 += 4 * dm) {
+  for (int m0 = tid / outs; m0 < M; m0 += 4 * dm) {
     float v[4];
     uint32_t mask[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) mask[u] = m0 + u * dm < (int)M && whole ? ep.mask_at(m0 + u * dm, o) : 0u;
+    for (int u = 0; u < 4; ++u) mask[u] = m0 + u * dm < M && whole ? ep.mask_at(m_lo + m0 + u * dm, o) : 0u;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       v[u] = 0.0f;
-      if (m0 + u * dm < (int)M)
+      if (m0 + u * dm < M)
         for (int p = P - 1; p >= 0; --p)  // small pieces first
-          for (int k = 0; k < wk_n; ++k) v[u] += red[((w * wk_n + k) * rows + p * (int)M + m0 + u * dm) * 32 + col];
+          for (int k = 0; k < wk_n; ++k) v[u] += red[((w * wk_n + k) * rows + p * M + m0 + u * dm) * 32 + col];
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int m = m0 + u * dm;
-      if (m >= (int)M) break;
-      if (whole) ep.store(m, o, v[u], b, mask[u]);
-      else part[((int64_t)blockIdx.y * M + m) * O + o] = v[u];
+      if (m >= M) break;
+      if (whole) ep.store(m_lo + m, o, v[u], b, mask[u]);
+      else part[((int64_t)blockIdx.y * M_all + m_lo + m) * O + o] = v[u];
     }
   }
 }
@@ -219,9 +229,9 @@ template <typename T, bool VJP>
 static void launch_skinny(hipStream_t st, const SkinnyPlan &p, int64_t M, int64_t L, int64_t O, const T *X, int64_t ldx,
                           const void *codes, const void *exps, int64_t Np, int64_t kbs, float *part,
                           const Epilogue<T, VJP> &ep) {
-  const dim3 grid((unsigned)p.gx, (unsigned)p.splits);
+  const dim3 grid((unsigned)p.gx, (unsigned)p.splits, (unsigned)p.groups);
 #define GO(RT)                                                                                                            \
-  hipLaunchKernelGGL((skinny_kernel<T, VJP, RT>), grid, dim3(64 * SK_WAVES), 0, st, M, L, O, X, ldx,                    \
+  hipLaunchKernelGGL((skinny_kernel<T, VJP, RT>), grid, dim3(64 * SK_WAVES), 0, st, M, p.mg, L, O, X, ldx,              \
                      (const char *)codes, (const char *)exps, Np, kbs, p.wk, p.steps, p.chunk, (uint32_t)cdiv(int64_t(1) << 32, p.chunk / 4), part, ep)
   if (p.rt == 1) GO(1);
   else if (p.rt == 2) GO(2);

@@ -142,11 +142,22 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
 
 // pieces of a floating operand of this type
 static inline int pieces(int dtype) { return dtype == GPVAE_LB_F32 ? 3 : dtype == GPVAE_LB_F16 ? 2 : 1; }
-static int64_t w4_workspace(int dtype, int64_t M, int64_t L, int64_t O) {
+// Few rows (skinny.hpp) or many (tile.hpp)?  Few: one launch (two where the reduction is split), every group of 64 / P rows decodes
+// all codes; many: the operand is split into planes first (a launch; none for most bfloat16 operands) and 64 rows share a
+// decoded tile.  Measured on both sides, few / many in us: float32 128 x 1024 x 4096 13.8 / 19.3 (transposed 19.3 / 24.9),
+// 256 x 1024 x 4096 23.9 / 25.2 (31.2 / 29.1), 42 x 4096 x 32768 47.7 / 69.7 (77 / 80), 64 x 4096 x 32768 75 / 71 (168 / 82);
+// bfloat16 256 x 1024 x 4096 13.0 / 19.6 (21.6 / 18.0), 128 x 1024 x 4096 transposed 17.1 / 16.0, 100 x 4096 x 32768 61 / 55.
+static inline bool use_skinny(int P, int64_t M, int64_t L, int64_t O, bool vjp) {
+  const int64_t groups = cdiv(M, SK_MAXROWS / P);
+  if (groups <= (P == 1 ? 1 : 2)) return true;
+  const double work = (double)P * (double)M * (double)L * (double)O;
+  return P == 1 ? !vjp && groups <= 4 && work <= 0x1p30 : groups <= 16 && work <= 0x1p31;
+}
+static int64_t w4_workspace(int dtype, int64_t M, int64_t L, int64_t O, bool vjp) {
   if (!dtype_ok(dtype) || M < 1 || L < 1 || O < 1) return 0;
   const int P = pieces(dtype);
-  if (P * M <= SK_MAXROWS) {
-    const SkinnyPlan p = skinny_plan(P * M, L, O);
+  if (use_skinny(P, M, L, O, vjp)) {
+    const SkinnyPlan p = skinny_plan(P, M, L, O);
     return p.splits > 1 ? p.splits * M * O * 4 : 0;
   }
   const TilePlan p = tile_plan(P, M, L, O, false);
@@ -156,8 +167,8 @@ template <typename T, bool VJP>
 static void run_w4(hipStream_t st, int64_t M, int64_t L, int64_t O, const void *X, int64_t ldx, const void *codes,
                    const void *exps, int64_t Np, int64_t kbs, void *work, const Epilogue<T, VJP> &ep) {
   constexpr int P = Split<T>::P;
-  if (P * M <= SK_MAXROWS) {
-    launch_skinny<T, VJP>(st, skinny_plan(P * M, L, O), M, L, O, (const T *)X, ldx, codes, exps, Np, kbs, (float *)work, ep);
+  if (use_skinny(P, M, L, O, VJP)) {
+    launch_skinny<T, VJP>(st, skinny_plan(P, M, L, O), M, L, O, (const T *)X, ldx, codes, exps, Np, kbs, (float *)work, ep);
   } else {
     // a bfloat16 operand is its own plane where its rows can be read 16 bytes at a time to the end of the last step and
     // 256 of them lie within a 32-bit offset
@@ -167,10 +178,10 @@ static void run_w4(hipStream_t st, int64_t M, int64_t L, int64_t O, const void *
   }
 }
 extern "C" int64_t gpvae_dense_w4_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
-  return w4_workspace(dtype, M, K, N);
+  return w4_workspace(dtype, M, K, N, false);
 }
 extern "C" int64_t gpvae_dense_vjp_w4_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
-  return w4_workspace(dtype, M, N, K);
+  return w4_workspace(dtype, M, N, K, true);
 }
 
 extern "C" int gpvae_dense_w4(void *stream, int dtype, int64_t M, int64_t K, int64_t N, const void *X, int64_t ldx,
@@ -187,7 +198,7 @@ extern "C" int gpvae_dense_w4(void *stream, int dtype, int64_t M, int64_t K, int
   LB_REQUIRE(exps && aligned16(exps), 9, "%s: exps must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(Y && Y != X, 12, "%s: Y is NULL or X", fn);
   LB_REQUIRE(ldy >= N, 13, "%s: ldy < N", fn);
-  LB_REQUIRE(!w4_workspace(dtype, M, K, N) || (work && aligned16(work)), 14, "%s: work must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(!w4_workspace(dtype, M, K, N, false) || (work && aligned16(work)), 14, "%s: work must be a 16-byte aligned device pointer", fn);
 #define GO(T)                                                                                                        \
   run_w4<T, false>((hipStream_t)stream, M, K, N, X, ldx, codes, exps, w4_np(N), w4_kb(K), work,                     \
                    Epilogue<T, false>{(const T *)bias, relu, nullptr, 0, (T *)Y, ldy})
@@ -212,7 +223,7 @@ extern "C" int gpvae_dense_vjp_w4(void *stream, int dtype, int64_t M, int64_t K,
   LB_REQUIRE(!act_codes || aligned16(act_codes), 10, "%s: act_codes must be 16-byte aligned", fn);
   LB_REQUIRE(dX && dX != dY, 11, "%s: dX is NULL or dY", fn);
   LB_REQUIRE(lddx >= K, 12, "%s: lddx < K", fn);
-  LB_REQUIRE(!w4_workspace(dtype, M, N, K) || (work && aligned16(work)), 13, "%s: work must be a 16-byte aligned device pointer", fn);
+  LB_REQUIRE(!w4_workspace(dtype, M, N, K, true) || (work && aligned16(work)), 13, "%s: work must be a 16-byte aligned device pointer", fn);
 #define GO(T)                                                                                                        \
   run_w4<T, true>((hipStream_t)stream, M, N, K, dY, lddy, codes, exps, w4_np(N), w4_kb(K), work,                    \
                   Epilogue<T, true>{nullptr, 0, (const uint8_t *)act_codes, q8_kp(K), (T *)dX, lddx})

@@ -123,7 +123,8 @@ def test_store_q8_special_values(relu):
 
 # ---- products ---------------------------------------------------------------------------------------------------------
 SHAPES = [(1, 50, 4096), (1, 1, 1), (2, 35, 300), (3, 300, 17), (16, 64, 128), (17, 1024, 65), (33, 31, 1000), (64, 100, 96),
-          (65, 700, 33), (100, 33, 625), (130, 257, 260), (256, 96, 129), (300, 513, 1030)]
+          (65, 700, 33), (100, 33, 625), (130, 257, 260), (256, 96, 129), (300, 513, 1030),
+          (22, 65, 97), (43, 130, 31), (350, 70, 99), (400, 129, 260), (1030, 65, 33), (515, 400, 640)]
 
 
 @pytest.mark.parametrize("dt", TYPES)
