@@ -159,12 +159,18 @@ __device__ __forceinline__ float sum_parts(const float *p, int64_t stride, int n
 template <typename T, bool VJP>
 __global__ __launch_bounds__(256) void split_sum_kernel(int64_t M, int64_t O, int splits, const float *__restrict__ part,
                                                         Epilogue<T, VJP> ep) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * O) return;
-  const int64_t m = i / O, o = i - m * O;
+  const int64_t o = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (o >= O) return;
   const float b = ep.bias_at(o);
-  const uint32_t mask = ep.mask_at(m, o);
-  ep.store(m, o, sum_parts(part + i, M * O, splits), b, mask);
+  for (int64_t m = blockIdx.y; m < M; m += gridDim.y) {
+    const uint32_t mask = ep.mask_at(m, o);
+    ep.store(m, o, sum_parts(part + m * O + o, M * O, splits), b, mask);
+  }
+}
+template <typename T, bool VJP>
+static void launch_split_sum(hipStream_t st, int64_t M, int64_t O, int splits, const float *part, const Epilogue<T, VJP> &ep) {
+  hipLaunchKernelGGL((split_sum_kernel<T, VJP>), dim3((unsigned)cdiv(O, 256), (unsigned)(M < 4096 ? M : 4096)), dim3(256), 0, st,
+                     M, O, splits, part, ep);
 }
 
 }  // namespace gpvae_lb

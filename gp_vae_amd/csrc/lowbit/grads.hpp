@@ -51,15 +51,16 @@ template <bool RELU> __device__ __forceinline__ u32x4 q8_frag(u32x2 q, uint32_t 
 template <typename T, bool RELU>
 __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t K, int64_t N, const char *__restrict__ codes,
                                                               const uint8_t *__restrict__ exps, const T *__restrict__ dY,
-                                                              int64_t lddy, int ktiles, int64_t s_all, int steps, float *dW,
+                                                              int64_t lddy, int ktiles, int s_all, int steps, float *dW,
                                                               int64_t lddw, float *db, int64_t part_stride) {
   constexpr int P = Split<T>::P, AB = 128 * 128, ST = AB * (1 + P);  // bytes of one image of 128 rows x 64; of a stage
   __shared__ __align__(16) unsigned char lds[2][ST];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave >> 2, wn = wave & 3, c = lane >> 4, l16 = lane & 15;  // wave: 64 rows of dW x 32 columns
   const int64_t bt = xcd_chunk(blockIdx.x, gridDim.x), kt = bt % ktiles, k0 = kt * 128, n0 = (bt / ktiles) * 128;
-  const int64_t s_lo = (int64_t)blockIdx.y * steps, s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
-  const int64_t Kp = q8_kp(K), mbs = q8_mb(M);
+  const int s_lo = (int)blockIdx.y * steps, s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
+  const int64_t Kp = q8_kp(K);
+  const int mbs = (int)q8_mb(M);
   const bool sum_db = db != nullptr && kt == 0;
   dW += blockIdx.y * part_stride;
   if (db) db += blockIdx.y * part_stride;
@@ -81,30 +82,34 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   };
   // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
   // may not have been issued does not count, so that the wait would reach into the step just issued.  Past the last step
-  // and the last row the last ones are read again.
-  auto issue = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
+  // and the last row the last ones are read again.  Addresses are scalar bases plus fixed lane offsets.
+  const int64_t rb = lddy * (int64_t)sizeof(T);
+  const char *const ybase = reinterpret_cast<const char *>(dY + n0);
+  auto issue = [&](Ahead &h, int s) __attribute__((always_inline)) {
     s = s < s_hi ? s : s_hi - 1;
-    const int64_t m = s * GR_ROWS + wave * 8;
+    const int m_ = s * GR_ROWS + wave * 8, m = __builtin_amdgcn_readfirstlane(m_ < (int)M ? m_ : (int)M - 1);
+    const int rem = (int)M - 1 - m;
+    const char *r = ybase + m * rb;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const char *row = reinterpret_cast<const char *>(dY + (m + i < M ? m + i : M - 1) * lddy + n0);
+      if (i) r += i <= rem ? rb : 0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) h.y[i][e] = *reinterpret_cast<const T *>(row + yoff[e]);
+      for (int e = 0; e < 2; ++e) h.y[i][e] = *reinterpret_cast<const T *>(r + yoff[e]);
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      int64_t mb = s * (GR_ROWS / 8) + xb + 4 * j;
-      mb = mb < mbs ? mb : mbs - 1;  // finite (or already NaN) times the zeros that put makes of rows past the last
+      int mb = s * (GR_ROWS / 8) + xb + 4 * j;
+      mb = __builtin_amdgcn_readfirstlane(mb < mbs ? mb : mbs - 1);  // finite (or already NaN) times the zeros that put makes of rows past the last
       h.q[j] = *reinterpret_cast<const u32x2 *>(codes + (mb * Kp + k0) * 8 + xoff);
-      h.e[j] = (exps + mb * (Kp / 8) + k0 / 8)[eoff];
+      h.e[j] = *(exps + (mb * Kp + k0) / 8 + eoff);
     }
   };
   float dbacc[2] = {0.0f, 0.0f};
-  auto put = [&](Ahead &h, int64_t s, int b) __attribute__((always_inline)) {
-    if ((s + 1) * GR_ROWS > M) {
+  auto put = [&](Ahead &h, int s, int b) __attribute__((always_inline)) {
+    if ((s + 1) * GR_ROWS > (int)M || s >= s_hi) {  // rows past the last, and a step past the last, add nothing
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (s * GR_ROWS + wave * 8 + i >= M) h.y[i][0] = h.y[i][1] = T(0.0f);
+        if (s * GR_ROWS + wave * 8 + i >= (int)M || s >= s_hi) h.y[i][0] = h.y[i][1] = T(0.0f);
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -118,7 +123,7 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
 #pragma unroll
     for (int j = 0; j < 2; ++j)
       *reinterpret_cast<u32x4 *>(lds[b] + xk * 128 + (((xb + 4 * j) ^ xsw) * 16)) = q8_frag<RELU>(h.q[j], h.e[j]);
-    if (sum_db && s < s_hi) {
+    if (sum_db) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -132,7 +137,7 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
 #pragma unroll
     for (int i = 0; i < 2; ++i) acc[a][i] = f32x4_t{0, 0, 0, 0};
   const int arow = (wk * 64 + l16) * 128, brow = AB + (wn * 32 + l16) * 128, sw = l16 >> 1;
-  auto step = [&](Ahead &now, Ahead &next, int64_t s, int b) __attribute__((always_inline)) {
+  auto step = [&](Ahead &now, Ahead &next, int s, int b) __attribute__((always_inline)) {
     u32x4 x[2][4], y[2][P][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -163,9 +168,12 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
     put(h0, s_lo, 0);
   }
   __syncthreads();
-  for (int64_t s = s_lo; s < s_hi; s += 2) {
+  // two steps a turn whatever their number (a step past the last adds zeros): a loop that may leave after the first makes the
+  // compiler copy registers whose loads are in flight, and wait for them
+#pragma unroll 1
+  for (int s = s_lo; s < s_hi; s += 2) {
     step(h0, h1, s, 0);
-    if (s + 1 < s_hi) step(h1, h0, s + 1, 1);
+    step(h1, h0, s + 1, 1);
   }
 #pragma unroll
   for (int a = 0; a < 4; ++a)
@@ -196,12 +204,13 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
 // partial sums [splits][K + 1][N] (the last row: db) -> dW, db, in order
 static __global__ __launch_bounds__(256) void grads_sum_kernel(int64_t K, int64_t N, int splits, const float *__restrict__ part,
                                                                float *__restrict__ dW, int64_t lddw, float *__restrict__ db) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (K + 1) * N;
-  if (i >= (db ? all : K * N)) return;
-  const float v = sum_parts(part + i, all, splits);
-  const int64_t k = i / N, n = i - k * N;
-  if (k < K) dW[k * lddw + n] = v;
-  else db[n] = v;
+  const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (n >= N) return;
+  for (int64_t k = blockIdx.y; k < (db ? K + 1 : K); k += gridDim.y) {
+    const float v = sum_parts(part + k * N + n, (K + 1) * N, splits);
+    if (k < K) dW[k * lddw + n] = v;
+    else db[n] = v;
+  }
 }
 
 template <typename T, bool RELU>
@@ -210,10 +219,10 @@ static void launch_grads(hipStream_t st, const GradsPlan &p, int64_t M, int64_t 
   const bool split = p.splits > 1;
   const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
   hipLaunchKernelGGL((grads_kernel<T, RELU>), grid, dim3(GR_THREADS), 0, st, M, K, N, (const char *)codes,
-                     (const uint8_t *)exps, dY, lddy, p.ktiles, cdiv(M, GR_ROWS), p.steps, split ? work : dW,
+                     (const uint8_t *)exps, dY, lddy, p.ktiles, (int)cdiv(M, GR_ROWS), p.steps, split ? work : dW,
                      split ? N : lddw, split ? (db ? work + K * N : nullptr) : db, split ? (K + 1) * N : 0);
   if (split)
-    hipLaunchKernelGGL(grads_sum_kernel, dim3((unsigned)cdiv((K + 1) * N, 256)), dim3(256), 0, st, K, N, p.splits, work, dW, lddw, db);
+    hipLaunchKernelGGL(grads_sum_kernel, dim3((unsigned)cdiv(N, 256), (unsigned)(K < 4096 ? K + 1 : 4096)), dim3(256), 0, st, K, N, p.splits, work, dW, lddw, db);
 }
 
 }  // namespace gpvae_lb

@@ -239,7 +239,7 @@ static void launch_skinny(hipStream_t st, const SkinnyPlan &p, int64_t M, int64_
   else GO(4);
 #undef GO
   if (p.splits > 1)
-    hipLaunchKernelGGL((split_sum_kernel<T, VJP>), dim3((unsigned)cdiv(M * O, 256)), dim3(256), 0, st, M, O, p.splits, part, ep);
+    launch_split_sum<T, VJP>(st, M, O, p.splits, part, ep);
 }
 
 }  // namespace gpvae_lb

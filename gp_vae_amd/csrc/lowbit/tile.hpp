@@ -10,14 +10,15 @@
 
 namespace gpvae_lb {
 
-// planes[p][k / 64][m][k % 64] of X [M, ldx], zero past L (Lp a multiple of 64): what a step stages is contiguous
+// planes[p][k / 64][m][k % 64] of X [M, ldx], zero past L (Lp a multiple of 128): what a step stages is contiguous.
+// A block of 256 threads takes 256 >> qsh rows (blockIdx.x) x 1024 columns (blockIdx.y), 4 elements a thread.
 template <typename T>
-__global__ __launch_bounds__(256) void split_planes_kernel(int64_t M, int64_t L, int64_t Lp, const T *__restrict__ X, int64_t ldx,
+__global__ __launch_bounds__(256) void split_planes_kernel(int64_t M, int64_t L, int64_t Lp, int qsh, const T *__restrict__ X, int64_t ldx,
                                                            u32x2 *__restrict__ planes) {
   constexpr int P = Split<T>::P;
-  const int64_t q = Lp / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * q) return;
-  const int64_t m = i / q, k4 = i - m * q;
+  const int64_t q = Lp / 4, m = ((int64_t)blockIdx.x << (8 - qsh)) + (threadIdx.x >> qsh);
+  const int64_t k4 = (int64_t)blockIdx.y * 256 + (threadIdx.x & ((1 << qsh) - 1));
+  if (m >= M || k4 >= q) return;
   const Vec4<T> v = load4(X + m * ldx, k4 * 4, L);
   uint32_t a[P], b[P];
   Split<T>::two(v.v[0], v.v[1], a);
@@ -74,6 +75,7 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
     }
   }
   const int64_t kbv0 = VJP ? (o0 / 32 < kbs ? o0 / 32 : kbs - 1) : 0, kbv1 = VJP ? (o0 / 32 + 1 < kbs ? o0 / 32 + 1 : kbs - 1) : 0;
+  const int64_t s_codes = VJP ? (Np - 1) / 64 : (kbs - 1) / 2;
   struct Ahead {  // what is in flight for a step: its share of the stage, its codes and tile exponents
     u32x4 st[NLD];
     u32x2 cw[4];
@@ -87,9 +89,10 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
     const char *const b = pbase + s * ss;
 #pragma unroll
     for (int i = 0; i < NLD; ++i) h.st[i] = *reinterpret_cast<const u32x4 *>(b + (i / NR) * ps + src[i % NR]);
+    const int64_t sc = s < s_codes ? s : s_codes;  // the planes may go on past the last step with codes
     if (!VJP) {
-      const char *const cb = codes + 2 * s * Np * 16, *const eb = exps + 2 * s * (Np / 2);
-      const bool odd = 2 * s + 1 >= kbs;  // the last block has no second one: lane groups 2, 3 read the first again
+      const char *const cb = codes + 2 * sc * Np * 16, *const eb = exps + 2 * sc * (Np / 2);
+      const bool odd = 2 * sc + 1 >= kbs;  // the last block has no second one: lane groups 2, 3 read the first again
       const uint32_t back_c = odd && c >= 2 ? (uint32_t)(Np * 16) : 0u, back_e = odd && c >= 2 ? (uint32_t)(Np / 2) : 0u;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
@@ -98,13 +101,13 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
       }
     } else {
       // columns 64 s + 32 (t / 2) ...: a second half past the end repeats the first
-      const uint32_t back = s * 64 + 32 >= Np ? 32u : 0u;
+      const uint32_t back = sc * 64 + 32 >= Np ? 32u : 0u;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int64_t kb = t & 1 ? kbv1 : kbv0;
         const uint32_t bk = t >> 1 ? back : 0u;
-        h.cw[t] = *reinterpret_cast<const u32x2 *>(codes + (kb * Np + s * 64) * 16 + (coff[t] - bk * 16));
-        h.ce[t] = *reinterpret_cast<const uint32_t *>(exps + (kb * Np + s * 64) / 2 + (eoff[t] - bk / 2));
+        h.cw[t] = *reinterpret_cast<const u32x2 *>(codes + (kb * Np + sc * 64) * 16 + (coff[t] - bk * 16));
+        h.ce[t] = *reinterpret_cast<const uint32_t *>(exps + (kb * Np + sc * 64) / 2 + (eoff[t] - bk / 2));
       }
     }
   };
@@ -153,21 +156,16 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[a][i] = mfma(x[t][p][a], f[t][i], acc[a][i]);
     };
-    // the compiler alone reads two fragments, waits, multiplies, and so on: all of a half step's fragments are read before
-    // the previous half is multiplied, and its decoding runs between that half's matrix instructions
+    // The codes are decoded before the loads that replace them are issued (else those go to other registers and are copied, and
+    // waited for, at the end of the turn), and a half step's fragments are read before the other half is multiplied.
     read(0);
-    issue(now, s + 2);
     decode(0);
+    decode(1);
     __builtin_amdgcn_sched_barrier(0);
+    issue(now, s + 2);
     read(1);
     __builtin_amdgcn_sched_barrier(0);
-    decode(1);
     multiply(0);
-#pragma unroll
-    for (int i = 0; i < P * MT * 4; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one matrix instruction
-      __builtin_amdgcn_sched_group_barrier(0x002, VJP ? 4 : 2, 0);  // vector instructions
-    }
     __builtin_amdgcn_sched_barrier(0);
     multiply(1);
     put(next, b ^ 1);
@@ -178,9 +176,12 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
   issue(h1, s_lo + 1);
   put(h0, 0);
   __syncthreads();
+  // an even number of steps: a loop that may leave after the first of two makes the compiler copy registers whose loads are in
+  // flight, and wait for them
+#pragma unroll 1
   for (int64_t s = s_lo; s < s_hi; s += 2) {
     step(h0, h1, s, 0);
-    if (s + 1 < s_hi) step(h1, h0, s + 1, 1);
+    step(h1, h0, s + 1, 1);
   }
   const bool whole = gridDim.y == 1;
   int64_t oi[4];
@@ -224,14 +225,14 @@ static inline TilePlan tile_plan(int P, int64_t M, int64_t L, int64_t O, bool di
   p.direct = direct;
   p.wm = 2;
   p.mt = 2;
-  p.Lp = round_up(L, 64);
+  p.Lp = round_up(L, 128);
   p.mtiles = (int)cdiv(M, 16 * p.mt * p.wm);
   p.blocks = p.mtiles * cdiv(O, 128);
   const int64_t steps = p.Lp / 64;
   int64_t s = p.blocks < 192 ? cdiv(256, p.blocks) : 1;
   if (s > steps / 4) s = steps / 4;
   if (s < 1) s = 1;
-  p.steps = (int)cdiv(steps, s);
+  p.steps = (int)round_up(cdiv(steps, s), 2);
   p.splits = (int)cdiv(steps, p.steps);
   p.plane_bytes = direct ? 0 : round_up(P * M * p.Lp * 2, 256);
   return p;
@@ -244,8 +245,10 @@ static void launch_tile(hipStream_t st, const TilePlan &p, int64_t M, int64_t L,
   const char *planes = reinterpret_cast<const char *>(X);
   int64_t rs = ldx * 2, ss = 128, ps = 0;
   if (!p.direct) {
-    hipLaunchKernelGGL((split_planes_kernel<T>), dim3((unsigned)cdiv(M * p.Lp / 4, 256)), dim3(256), 0, st, M, L, p.Lp, X, ldx,
-                       (u32x2 *)work);
+    int qsh = 5;  // 2^qsh >= Lp / 4, at most 256 threads to a row
+    while (qsh < 8 && (4 << qsh) < p.Lp) ++qsh;
+    hipLaunchKernelGGL((split_planes_kernel<T>), dim3((unsigned)cdiv(M, 256 >> qsh), (unsigned)cdiv(p.Lp, 1024)), dim3(256), 0, st,
+                       M, L, p.Lp, qsh, X, ldx, (u32x2 *)work);
     planes = reinterpret_cast<const char *>(work);
     rs = 128, ss = M * 128, ps = M * p.Lp * 2;
   }
@@ -258,7 +261,7 @@ static void launch_tile(hipStream_t st, const TilePlan &p, int64_t M, int64_t L,
   else GO(4, 2);
 #undef GO
   if (p.splits > 1)
-    hipLaunchKernelGGL((split_sum_kernel<T, VJP>), dim3((unsigned)cdiv(M * O, 256)), dim3(256), 0, st, M, O, p.splits, part, ep);
+    launch_split_sum<T, VJP>(st, M, O, p.splits, part, ep);
 }
 
 }  // namespace gpvae_lb

@@ -172,7 +172,7 @@ static void run_w4(hipStream_t st, int64_t M, int64_t L, int64_t O, const void *
   } else {
     // a bfloat16 operand is its own plane where its rows can be read 16 bytes at a time to the end of the last step and
     // 256 of them lie within a 32-bit offset
-    const bool direct = P == 1 && L % 64 == 0 && ldx % 8 == 0 && ldx < (1 << 23) && aligned16(X);
+    const bool direct = P == 1 && L % 128 == 0 && ldx % 8 == 0 && ldx < (1 << 23) && aligned16(X);
     launch_tile<T, VJP>(st, tile_plan(P, M, L, O, direct), M, L, O, (const T *)X, ldx, codes, exps, Np, kbs,
                         (unsigned char *)work, ep);
   }
