@@ -1,4 +1,4 @@
-// tile.hpp — the products of skinny.hpp for many rows: tiles of (16 MT WM) rows x 128 outputs on the bf16 matrix pipe.
+// tile.hpp — the products of skinny.hpp for many rows: tiles of 64 rows x 128 outputs on the bf16 matrix pipe.
 //
 // Bound by the matrix pipe (2 M K N flop per piece), so the loop must feed it: the floating operand is split into its
 // planes ONCE by split_planes_kernel (a workgroup splitting its own rows would repeat that for every 128 outputs, and
@@ -27,16 +27,17 @@ __global__ __launch_bounds__(256) void split_planes_kernel(int64_t M, int64_t L,
   for (int p = 0; p < P; ++p) planes[p * M * q + ((k4 >> 4) * M + m) * 16 + (k4 & 15)] = u32x2{a[p], b[p]};
 }
 
-// WM x 2 waves, each 16 MT rows x 64 outputs
+constexpr int TL_WM = 2, TL_MT = 2;  // TL_WM x 2 waves, each 16 TL_MT rows x 64 outputs
+
 // Addresses are a scalar base that moves with the step plus a fixed 32-bit offset per lane, so that the loop spends no vector
 // instruction on them.  Operand element (piece p, row m, reduction index k) is at byte p ps + (k / 64) ss + m rs + 2 (k % 64).
-template <typename T, bool VJP, int WM, int MT>
-__global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O, const char *__restrict__ planes, int64_t rs,
+template <typename T, bool VJP>
+__global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t O, const char *__restrict__ planes, int64_t rs,
                                                            int64_t ss, int64_t ps, const char *__restrict__ codes,
                                                            const char *__restrict__ exps, int64_t Np, int64_t kbs, int mtiles,
                                                            int64_t s_all, int steps, float *__restrict__ part,
                                                            Epilogue<T, VJP> ep) {
-  constexpr int P = Split<T>::P, NT = 128 * WM, BM = 16 * MT * WM;
+  constexpr int P = Split<T>::P, WM = TL_WM, MT = TL_MT, NT = 128 * WM, BM = 16 * MT * WM;
   constexpr int CH = P * BM * 8, NLD = CH / NT;  // 16-byte chunks of a stage, and of one thread's share
   static_assert(BM % (NT / 8) == 0 && NT / 8 % 8 == 0, "whole shares");
   __shared__ __align__(16) unsigned char lds[2][CH * 16];
@@ -58,7 +59,10 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
     src[i] = (uint32_t)((m0 + row < M ? row : M - 1 - m0) * rs) + ck8 * 16;  // rows past the last: results unused
   }
   const char *const pbase = planes + m0 * rs;
-  const int dst = (trow * 8 + (ck8 ^ ((trow >> 1) & 7))) * 16;
+  // lane group c reads chunk 2 c + t (product) or 4 t + c: either is kept at 4 t + c, so that the reads of the lane groups that
+  // share a cycle never meet in a bank
+  const int pk8 = VJP ? ck8 : (ck8 >> 1) | (ck8 & 1) << 2;
+  const int dst = (trow * 8 + (pk8 ^ ((trow >> 1) & 7))) * 16;
   // codes of one step: product: 8 bytes (two groups of 8 rows) of each of 4 columns 16 apart, lane group c taking rows
   // 32 (c / 2) + 16 (c % 2) + ...; transposed product: 8 bytes of a column for two blocks of 32 columns x two of 32 rows.
   // Past the ends the last codes are read again: their outputs are unused, or they meet the operand's zeros.
@@ -130,7 +134,7 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
     for (int t = 0; t < 4; ++t) w[t] = now.cw[t], e[t] = now.ce[t] >> (16 * (VJP ? half : c & 1));
     u32x4 x[2][P][MT], f[2][4];
     auto read = [&](int t) __attribute__((always_inline)) {
-      const int ck = ((VJP ? t * 4 + c : 2 * c + t) ^ sw) * 16;
+      const int ck = ((t * 4 + c) ^ sw) * 16;
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)
 #pragma unroll
@@ -214,26 +218,34 @@ __global__ __launch_bounds__(128 * WM, 2) void tile_kernel(int64_t M, int64_t O,
 }
 
 struct TilePlan {
-  int wm, mt;          // kernel shape
   int mtiles, splits, steps;
   int64_t blocks, Lp, plane_bytes;
   bool direct;         // the operand itself is its only plane
 };
 
+// Into how many parts is the reduction split?  A step of 64 takes 0.27 + 0.24 P us where a compute unit has one workgroup and
+// 0.23 + 0.35 P us where it has the two that fit, every full round of 512 workgroups anew; a split costs the launch that adds
+// the parts (4 us) and writing and reading them.  The least of that estimate over powers of two and the numbers that give
+// every unit one or two workgroups.  Measured, one part / two / four: float32 512 x 4096 x 4096 78 / 65 us, 512 x 1024 x 4096
+// 28.2 / 33.5; float32 1024 x 1024 x 4096 transposed - / 59 / 51; bfloat16 1024 x 1000 x 1000 17.2 / 22.1.
 static inline TilePlan tile_plan(int P, int64_t M, int64_t L, int64_t O, bool direct) {
   TilePlan p;
   p.direct = direct;
-  p.wm = 2;
-  p.mt = 2;
   p.Lp = round_up(L, 128);
-  p.mtiles = (int)cdiv(M, 16 * p.mt * p.wm);
+  p.mtiles = (int)cdiv(M, 16 * TL_MT * TL_WM);
   p.blocks = p.mtiles * cdiv(O, 128);
   const int64_t steps = p.Lp / 64;
-  int64_t s = p.blocks < 192 ? cdiv(256, p.blocks) : 1;
-  if (s > steps / 4) s = steps / 4;
-  if (s < 1) s = 1;
-  p.steps = (int)round_up(cdiv(steps, s), 2);
-  p.splits = (int)cdiv(steps, p.steps);
+  p.splits = 1;
+  p.steps = (int)steps;
+  double best = 0.0;
+  for (int64_t i = 1; i <= 512; i *= 2)
+    for (int64_t s : {i, i < 256 ? int64_t(0) : 256 * (i / 256) / p.blocks}) {
+      if (s < 1 || (s > 1 && (s * p.blocks > 640 || s * 4 > steps))) continue;
+      const int64_t per = round_up(cdiv(steps, s), 2), parts = cdiv(steps, per), b = parts * p.blocks;
+      const double step = b <= 256 ? 0.27 + 0.24 * P : (double)cdiv(b, 512) * (0.23 + 0.35 * P);
+      const double t = (double)per * step + (parts > 1 ? 4.0 + (double)parts * ((double)M * (double)O * (8 / 4.5e6) + 0.06) : 0.0);
+      if (s == 1 || t < best) best = t, p.splits = (int)parts, p.steps = (int)per;
+    }
   p.plane_bytes = direct ? 0 : round_up(P * M * p.Lp * 2, 256);
   return p;
 }
@@ -254,12 +266,8 @@ static void launch_tile(hipStream_t st, const TilePlan &p, int64_t M, int64_t L,
   }
   float *part = reinterpret_cast<float *>(work + p.plane_bytes);
   const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
-#define GO(WM, MT)                                                                                                        \
-  hipLaunchKernelGGL((tile_kernel<T, VJP, WM, MT>), grid, dim3(128 * WM), 0, st, M, O, planes, rs, ss, ps,              \
-                     (const char *)codes, (const char *)exps, Np, kbs, p.mtiles, p.Lp / 64, p.steps, part, ep)
-  if (p.wm == 2) GO(2, 2);
-  else GO(4, 2);
-#undef GO
+  hipLaunchKernelGGL((tile_kernel<T, VJP>), grid, dim3(128 * TL_WM), 0, st, M, O, planes, rs, ss, ps, (const char *)codes,
+                     (const char *)exps, Np, kbs, p.mtiles, p.Lp / 64, p.steps, part, ep);
   if (p.splits > 1)
     launch_split_sum<T, VJP>(st, M, O, p.splits, part, ep);
 }
