@@ -4,10 +4,13 @@
 // The reduction runs over the ROWS of both operands, the matrix instruction wants 8 consecutive reduction indices per lane.
 // The checkpoint is laid out for that (8 rows of a column are 8 consecutive bytes); dY is transposed on its way into
 // LDS: a thread loads 8 consecutive rows of a column (consecutive lanes: consecutive columns), splits them into their
-// bfloat16 pieces and writes each piece's 8 values as 16 bytes.  Bound by the matrix pipe and LDS (one 128 x 128
-// tile per workgroup, 64 rows a step): the conversions are vector work that is dealt between the matrix instructions of
-// the step before.  All row tiles of a column tile run on one XCD (xcd_chunk), whose L2 then serves dY to them: dealt
-// round-robin every XCD read all of dY from memory (4096 x 1024 x 4096 float32: 140 us; with it see the launch).
+// bfloat16 pieces and writes each piece's 8 values as 16 bytes.  One 128 x 128 tile per workgroup, 64 rows a step, loaded
+// one step ahead through buffer descriptors: scalar bases, and rows and columns past the ends read as zero without a test.
+// Matrix and vector instructions of a SIMD take turns, so their sum bounds float32 (4096 x 1024 x 4096: matrix pipe 43 % of the
+// time, vector 48 %; 107 us, 965 TFLOP/s over the three pieces); bfloat16 also waits for LDS and the step's barrier (61 us,
+// float16 85 us; a library product of two bfloat16 matrices of this size: 52 us).  All row tiles of a column tile
+// run on one XCD (xcd_chunk), whose L2 then serves dY to them: dealt round-robin every XCD read all of dY from memory
+// (140 us before, 122 after).  Tried without gain: 4 steps in flight, the two waves of a SIMD half a step apart.
 #pragma once
 #include "frag.hpp"
 
@@ -48,16 +51,53 @@ template <bool RELU> __device__ __forceinline__ u32x4 q8_frag(u32x2 q, uint32_t 
   return u32x4{pack_hi(v[0], v[1]), pack_hi(v[2], v[3]), pack_hi(v[4], v[5]), pack_hi(v[6], v[7])};
 }
 
-template <typename T, bool RELU>
+// A buffer of `bytes` at a wave-uniform base: what lies past it reads as zero, without an access.
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t buffer(const char *base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, bytes, 0x00027000);
+}
+
+// What a thread has loaded of dY for a step: 8 rows of two columns, which are lane and lane + 64, or, for two-byte types (PAIR),
+// 2 lane and 2 lane + 1 with one load for both.
+template <typename T, bool PAIR> struct RowsOf {
+  uint32_t w[8][PAIR ? 1 : 2];
+  __device__ __forceinline__ void load(rsrc_t r, int i, int lane) {
+    if constexpr (PAIR) {
+      w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, 0, 0);
+    } else if constexpr (sizeof(T) == 4) {
+      w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, 0, 0);
+      w[i][1] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4 + 256, 0, 0);
+    } else {
+      w[i][0] = __builtin_amdgcn_raw_buffer_load_b16(r, lane * 2, 0, 0);
+      w[i][1] = __builtin_amdgcn_raw_buffer_load_b16(r, lane * 2 + 128, 0, 0);
+    }
+  }
+  __device__ __forceinline__ T value(int i, int e) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, w[i][e]);
+    else if constexpr (PAIR) return __builtin_bit_cast(T, (uint16_t)(w[i][0] >> (16 * e)));
+    else return __builtin_bit_cast(T, (uint16_t)w[i][e]);
+  }
+  // rows i and i + 1 of a column -> one dword of each piece
+  __device__ __forceinline__ void split(int i, int e, uint32_t *out) const {
+    if constexpr (__is_same(T, __bf16))
+      out[0] = PAIR ? __builtin_amdgcn_perm(w[i + 1][0], w[i][0], e ? 0x07060302u : 0x05040100u)
+                    : __builtin_amdgcn_perm(w[i + 1][e], w[i][e], 0x05040100u);
+    else Split<T>::two(value(i, e), value(i + 1, e), out);
+  }
+};
+
+template <typename T, bool RELU, bool PAIR>
 __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t K, int64_t N, const char *__restrict__ codes,
-                                                              const uint8_t *__restrict__ exps, const T *__restrict__ dY,
+                                                              const char *__restrict__ exps, const T *__restrict__ dY,
                                                               int64_t lddy, int ktiles, int s_all, int steps, float *dW,
                                                               int64_t lddw, float *db, int64_t part_stride) {
   constexpr int P = Split<T>::P, AB = 128 * 128, ST = AB * (1 + P);  // bytes of one image of 128 rows x 64; of a stage
   __shared__ __align__(16) unsigned char lds[2][ST];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wk = wave >> 2, wn = wave & 3, c = lane >> 4, l16 = lane & 15;  // wave: 64 rows of dW x 32 columns
-  const int64_t bt = xcd_chunk(blockIdx.x, gridDim.x), kt = bt % ktiles, k0 = kt * 128, n0 = (bt / ktiles) * 128;
+  const uint32_t bt = (uint32_t)xcd_chunk(blockIdx.x, gridDim.x);
+  const uint32_t nt = __builtin_amdgcn_readfirstlane(bt / (uint32_t)ktiles), kt = bt - nt * (uint32_t)ktiles;
+  const int64_t k0 = (int64_t)kt * 128, n0 = (int64_t)nt * 128;
   const int s_lo = (int)blockIdx.y * steps, s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
   const int64_t Kp = q8_kp(K);
   const int mbs = (int)q8_mb(M);
@@ -65,60 +105,46 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   dW += blockIdx.y * part_stride;
   if (db) db += blockIdx.y * part_stride;
 
-  // dY share: columns lane and lane + 64, rows 8 wave .. + 7 of the step; checkpoint share: column tid % 128, blocks of
-  // 8 rows tid / 128 and + 4.  Past the last column (row of dW): the last one again, results unused.
-  uint32_t yoff[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) yoff[e] = (uint32_t)((n0 + lane + 64 * e < N ? lane + 64 * e : N - 1 - n0) * sizeof(T));
+  // dY share: two columns, rows 8 wave .. + 7 of the step; checkpoint share: column tid % 128, blocks of 8 rows tid / 128 and
+  // + 4.  Everything outside the matrices, and a step past the last, is loaded as zero.
   const int xk = tid & 127, xb = wave >> 1;
-  const int64_t kk = k0 + xk < Kp ? k0 + xk : Kp - 1;
-  const uint32_t xoff = (uint32_t)(kk - k0) * 8, eoff = (uint32_t)(kk / 8 - k0 / 8);
-  const int ydst = AB + lane * 128 + ((wave ^ ((lane >> 1) & 7)) * 16);   // lane + 64: same swizzle
+  const int ycol0 = PAIR ? 2 * lane : lane, ycol1 = PAIR ? ycol0 + 1 : lane + 64;
+  const int ydst0 = AB + ycol0 * 128 + ((wave ^ ((ycol0 >> 1) & 7)) * 16), ydst1 = ydst0 + (ycol1 - ycol0) * 128;  // same swizzle
   const int xsw = (xk >> 1) & 7;
   struct Ahead {
-    T y[8][2];
+    RowsOf<T, PAIR> y;
     u32x2 q[2];
     uint32_t e[2];
   };
   // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
-  // may not have been issued does not count, so that the wait would reach into the step just issued.  Past the last step
-  // and the last row the last ones are read again.  Addresses are scalar bases plus fixed lane offsets.
+  // may not have been issued does not count, so that the wait would reach into the step just issued.
   const int64_t rb = lddy * (int64_t)sizeof(T);
   const char *const ybase = reinterpret_cast<const char *>(dY + n0);
+  const int ybytes = (int)(N - n0 < 128 ? N - n0 : 128) * (int)sizeof(T), xcols = (int)(Kp - k0 < 128 ? Kp - k0 : 128);
   auto issue = [&](Ahead &h, int s) __attribute__((always_inline)) {
-    s = s < s_hi ? s : s_hi - 1;
-    const int m_ = s * GR_ROWS + wave * 8, m = __builtin_amdgcn_readfirstlane(m_ < (int)M ? m_ : (int)M - 1);
-    const int rem = (int)M - 1 - m;
-    const char *r = ybase + m * rb;
+    const int m = s * GR_ROWS + wave * 8, rows = s < s_hi ? (int)M - m : 0;
+    const char *const r = ybase + m * rb;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i) r += i <= rem ? rb : 0;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) h.y[i][e] = *reinterpret_cast<const T *>(r + yoff[e]);
-    }
+    for (int i = 0; i < 8; ++i) h.y.load(buffer(r + i * rb, i < rows ? ybytes : 0), i, lane);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      int mb = s * (GR_ROWS / 8) + xb + 4 * j;
-      mb = __builtin_amdgcn_readfirstlane(mb < mbs ? mb : mbs - 1);  // finite (or already NaN) times the zeros that put makes of rows past the last
-      h.q[j] = *reinterpret_cast<const u32x2 *>(codes + (mb * Kp + k0) * 8 + xoff);
-      h.e[j] = *(exps + (mb * Kp + k0) / 8 + eoff);
+      const int mb = s * (GR_ROWS / 8) + xb + 4 * j;
+      const bool in = s < s_hi && mb < mbs;
+      const int64_t at = mb * Kp + k0;
+      h.q[j] = __builtin_amdgcn_raw_buffer_load_b64(buffer(codes + at * 8, in ? xcols * 8 : 0), xk * 8, 0, 0);
+      h.e[j] = __builtin_amdgcn_raw_buffer_load_b8(buffer(exps + at / 8, in ? xcols / 8 : 0), xk / 8, 0, 0);
     }
   };
   float dbacc[2] = {0.0f, 0.0f};
-  auto put = [&](Ahead &h, int s, int b) __attribute__((always_inline)) {
-    if ((s + 1) * GR_ROWS > (int)M || s >= s_hi) {  // rows past the last, and a step past the last, add nothing
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (s * GR_ROWS + wave * 8 + i >= (int)M || s >= s_hi) h.y[i][0] = h.y[i][1] = T(0.0f);
-    }
+  auto put = [&](const Ahead &h, int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       uint32_t w[4][P];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) Split<T>::two(h.y[2 * i][e], h.y[2 * i + 1][e], w[i]);
+      for (int i = 0; i < 4; ++i) h.y.split(2 * i, e, w[i]);
 #pragma unroll
       for (int p = 0; p < P; ++p)
-        *reinterpret_cast<u32x4 *>(lds[b] + ydst + p * AB + e * 64 * 128) = u32x4{w[0][p], w[1][p], w[2][p], w[3][p]};
+        *reinterpret_cast<u32x4 *>(lds[b] + (e ? ydst1 : ydst0) + p * AB) = u32x4{w[0][p], w[1][p], w[2][p], w[3][p]};
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -127,7 +153,7 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) dbacc[e] += to_f32(h.y[i][e]);
+        for (int i = 0; i < 8; ++i) dbacc[e] += to_f32(h.y.value(i, e));
     }
   };
 
@@ -137,7 +163,7 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
 #pragma unroll
     for (int i = 0; i < 2; ++i) acc[a][i] = f32x4_t{0, 0, 0, 0};
   const int arow = (wk * 64 + l16) * 128, brow = AB + (wn * 32 + l16) * 128, sw = l16 >> 1;
-  auto step = [&](Ahead &now, Ahead &next, int s, int b) __attribute__((always_inline)) {
+  auto multiply = [&](int b) __attribute__((always_inline)) {
     u32x4 x[2][4], y[2][P][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -149,7 +175,6 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
 #pragma unroll
         for (int i = 0; i < 2; ++i) y[t][p][i] = *reinterpret_cast<const u32x4 *>(lds[b] + brow + p * AB + i * 2048 + ck);
     }
-    issue(now, s + 2);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -158,14 +183,19 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
         for (int a = 0; a < 4; ++a)
 #pragma unroll
           for (int i = 0; i < 2; ++i) acc[a][i] = mfma(x[t][a], y[t][p][i], acc[a][i]);
-    put(next, s + 1, b ^ 1);
+  };
+  // Step s is in lds[b], `next` holds s + 1 in flight, s + 2 replaces `now`.
+  auto step = [&](Ahead &now, Ahead &next, int s, int b) __attribute__((always_inline)) {
+    issue(now, s + 2);
+    multiply(b);
+    put(next, b ^ 1);
     __syncthreads();
   };
   Ahead h0, h1;
   if (s_lo < s_hi) {
     issue(h0, s_lo);
     issue(h1, s_lo + 1);
-    put(h0, s_lo, 0);
+    put(h0, 0);
   }
   __syncthreads();
   // two steps a turn whatever their number (a step past the last adds zeros): a loop that may leave after the first makes the
@@ -189,8 +219,8 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
     }
   if (sum_db) {  // rows 8 wave .. of every step, added over the waves in order
     float *red = reinterpret_cast<float *>(lds);
-    red[wave * 128 + lane] = dbacc[0];
-    red[wave * 128 + 64 + lane] = dbacc[1];
+    red[wave * 128 + ycol0] = dbacc[0];
+    red[wave * 128 + ycol1] = dbacc[1];
     __syncthreads();
     if (tid < 128 && n0 + tid < N) {
       float v = 0.0f;
@@ -218,9 +248,19 @@ static void launch_grads(hipStream_t st, const GradsPlan &p, int64_t M, int64_t 
                          const void *exps, const T *dY, int64_t lddy, float *dW, int64_t lddw, float *db, float *work) {
   const bool split = p.splits > 1;
   const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
-  hipLaunchKernelGGL((grads_kernel<T, RELU>), grid, dim3(GR_THREADS), 0, st, M, K, N, (const char *)codes,
-                     (const uint8_t *)exps, dY, lddy, p.ktiles, (int)cdiv(M, GR_ROWS), p.steps, split ? work : dW,
-                     split ? N : lddw, split ? (db ? work + K * N : nullptr) : db, split ? (K + 1) * N : 0);
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(GR_THREADS), 0, st, M, K, N, (const char *)codes, (const char *)exps, dY, lddy,
+                       p.ktiles, (int)cdiv(M, GR_ROWS), p.steps, split ? work : dW, split ? N : lddw,
+                       split ? (db ? work + K * N : nullptr) : db, split ? (K + 1) * N : 0);
+  };
+  // Two-byte types: both columns of a pair exist or neither, and a pair is aligned to 4 bytes.  One load for two columns
+  // against two: bfloat16 4096 x 1024 x 4096 61.4 / 65.7 us.  (float32 in pairs gained nothing.)
+  if constexpr (sizeof(T) == 2) {
+    if (N % 2 == 0 && lddy % 2 == 0 && ((uintptr_t)dY & 3) == 0) launch(grads_kernel<T, RELU, true>);
+    else launch(grads_kernel<T, RELU, false>);
+  } else {
+    launch(grads_kernel<T, RELU, false>);
+  }
   if (split)
     hipLaunchKernelGGL(grads_sum_kernel, dim3((unsigned)cdiv(N, 256), (unsigned)(K < 4096 ? K + 1 : 4096)), dim3(256), 0, st, K, N, p.splits, work, dW, lddw, db);
 }
