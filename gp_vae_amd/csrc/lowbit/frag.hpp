@@ -98,6 +98,9 @@ template <> struct Split<__bf16> {
     out[0] = (uint32_t)__builtin_bit_cast(uint16_t, a) | ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
   }
 };
+// pieces of an operand of this type
+static inline int pieces(int dtype) { return dtype == GPVAE_LB_F32 ? 3 : dtype == GPVAE_LB_F16 ? 2 : 1; }
+
 // four elements at any element-aligned address: one vector load (unaligned access is on)
 template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Vec4 { T v[4]; };
 

@@ -176,7 +176,7 @@ extern "C" int gpvae_load_q8(void *stream, int dtype, int64_t M, int64_t K, int 
 
 extern "C" int64_t gpvae_dense_grads_q8_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
   if (!dtype_ok(dtype) || M < 0 || K < 1 || N < 1) return 0;
-  const GradsPlan p = grads_plan(M, K, N);
+  const GradsPlan p = grads_plan(pieces(dtype), M, K, N);
   return p.splits > 1 ? p.splits * (K + 1) * N * 4 : 0;
 }
 
@@ -194,7 +194,7 @@ extern "C" int gpvae_dense_grads_q8(void *stream, int dtype, int64_t M, int64_t 
   LB_REQUIRE(lddw >= N, 12, "%s: lddw < N", fn);
   LB_REQUIRE(!gpvae_dense_grads_q8_workspace_bytes(dtype, M, K, N) || (work && aligned16(work)), 14,
              "%s: work must be a 16-byte aligned device pointer", fn);
-  const GradsPlan p = grads_plan(M, K, N);
+  const GradsPlan p = grads_plan(pieces(dtype), M, K, N);
 #define GO2(T, R)                                                                                                       \
   launch_grads<T, R>((hipStream_t)stream, p, M, K, N, codes, exps, (const T *)dY, lddy, dW, lddw, db, (float *)work)
 #define GO(T) do { if (relu) GO2(T, true); else GO2(T, false); } while (0)

@@ -140,8 +140,6 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
   return 0;
 }
 
-// pieces of a floating operand of this type
-static inline int pieces(int dtype) { return dtype == GPVAE_LB_F32 ? 3 : dtype == GPVAE_LB_F16 ? 2 : 1; }
 // Few rows (skinny.hpp) or many (tile.hpp)?  Few: one launch (two where the reduction is split), every group of 64 / P rows decodes
 // all codes; many: the operand is split into planes first (a launch; none for most bfloat16 operands) and 64 rows share a
 // decoded tile.  Measured on both sides, few / many in us: float32 128 x 1024 x 4096 13.8 / 19.3 (transposed 19.3 / 24.9),
