@@ -140,16 +140,22 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
   return 0;
 }
 
-// Few rows (skinny.hpp) or many (tile.hpp)?  Few: one launch (two where the reduction is split), every group of 64 / P rows decodes
-// all codes; many: the operand is split into planes first (a launch; none for most bfloat16 operands) and 64 rows share a
-// decoded tile.  Measured on both sides, few / many in us: float32 128 x 1024 x 4096 13.8 / 19.3 (transposed 19.3 / 24.9),
-// 256 x 1024 x 4096 23.9 / 25.2 (31.2 / 29.1), 42 x 4096 x 32768 47.7 / 69.7 (77 / 80), 64 x 4096 x 32768 75 / 71 (168 / 82);
-// bfloat16 256 x 1024 x 4096 13.0 / 19.6 (21.6 / 18.0), 128 x 1024 x 4096 transposed 17.1 / 16.0, 100 x 4096 x 32768 61 / 55.
+// Few rows (skinny.hpp) or many (tile.hpp)?  Few: one launch (two where the reduction is split), every group of 64 / P rows
+// decodes all codes, every workgroup stages the operand anew; many: the operand is split into planes first (a launch; none for
+// most bfloat16 operands) and 64 rows share a decoded tile.  Measured on both sides, few / many in us (t: transposed):
+//   bfloat16 16 x 4096 x 32768 25 / 30 (t 37 / 37), 24 x 4096 x 32768 32 / 32 (t 47 / 38), 64 x 4096 x 32768 67 / 39 (t 64 / 41),
+//     64 x 1024 x 4096 12.4 / 11.5, 200 x 512 x 512 8.0 / 9.8, 128 x 512 x 512 t 10.2 / 12.4;
+//   float16 24 x 4096 x 32768 40 / 45 (t 45 / 48), 32 x 8192 x 8192 29 / 29 (t 32 / 32), 64 x 4096 x 32768 55 / 52 (t 92 / 52),
+//     200 x 1024 x 4096 14 / 21 (t 21.7 / 23.5), 96 x 4096 x 32768 94 / 68;
+//   float32 21 x 4096 x 32768 39 / 56 (t 46 / 61), 42 x 1024 x 32768 18 / 27 (t 28 / 36), 42 x 8192 x 8192 54 / 37 (t 60 / 41),
+//     42 x 4096 x 32768 47 / 59 (t 79 / 66), 256 x 1024 x 4096 23 / 26 (t 31 / 29), 128 x 4096 x 4096 34 / 28 (t 39 / 31).
 static inline bool use_skinny(int P, int64_t M, int64_t L, int64_t O, bool vjp) {
   const int64_t groups = cdiv(M, SK_MAXROWS / P);
-  if (groups <= (P == 1 ? 1 : 2)) return true;
   const double work = (double)P * (double)M * (double)L * (double)O;
-  return P == 1 ? !vjp && groups <= 4 && work <= 0x1p30 : groups <= 16 && work <= 0x1p31;
+  if (P == 1) return M <= 16 || (groups <= 4 && work <= 0x1p28);
+  if (groups == 1) return P == 3 || M <= 24 || work <= 0x1p32;
+  if (groups == 2) return work <= 0x1p32 || (P == 3 && !vjp && O >= 4 * L);
+  return groups <= 16 && work <= 3 * 0x1p30;
 }
 static int64_t w4_workspace(int dtype, int64_t M, int64_t L, int64_t O, bool vjp) {
   if (!dtype_ok(dtype) || M < 1 || L < 1 || O < 1) return 0;
