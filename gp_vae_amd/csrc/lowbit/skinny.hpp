@@ -138,6 +138,7 @@ __global__ __launch_bounds__(64 * SK_WAVES) void skinny_kernel(int64_t M_all, in
       };
       const T *const x0 = X + s0 * 128;
       if (s0 * 128 + chunk <= L) {
+#pragma unroll 2  // two vectors in flight: 21 x 4096 x 32768 float32 39.2 -> 34.6 us
         for (int i = tid; i < M * q; i += 64 * SK_WAVES) {
           const int m = (int)__umulhi((uint32_t)i, magic), k4 = i - m * q;
           put(m, k4, *reinterpret_cast<const Vec4<T> *>(x0 + m * ldx + k4 * 4));
