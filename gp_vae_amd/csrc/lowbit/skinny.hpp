@@ -28,15 +28,24 @@ static constexpr int skinny_lds(int rt) { return rt <= 1 ? 40 << 10 : rt == 2 ? 
 // P pieces of M rows, L reduction indices, O outputs
 static inline SkinnyPlan skinny_plan(int P, int64_t M, int64_t L, int64_t O) {
   SkinnyPlan p;
-  p.groups = (int)cdiv(M, SK_MAXROWS / P);
-  p.mg = (int)cdiv(M, p.groups);
-  const int rows = P * p.mg;
-  p.rt = (int)cdiv(rows, 16);
   const int64_t steps = cdiv(L, 128), tiles = cdiv(O, 32);
-  const int room = (int)((skinny_lds(p.rt) / rows - 16) / 256);  // steps whose image fits
-  p.wk = 1;
-  while (p.wk < SK_WAVES && 2 * p.wk <= steps && 2 * p.wk <= room && tiles * p.wk < 2048) p.wk *= 2;
-  p.gx = cdiv(tiles, SK_WAVES / p.wk);
+  // Smaller groups than fit where that leaves the chip idle: each decodes all codes again, but stages fewer rows.  Up to 256
+  // workgroups for a short reduction, 128 for a longer one; beyond, splitting the reduction is better.  Before / after: float32
+  // 37 x 700 x 1025 transposed 12.1 / 6.8 us, bfloat16 60 rows 13.3 / 7.7, 64 x 4000 x 200 14.1 / 10.9; where it is not
+  // done: float32 128 x 1024 x 4096 transposed 18.8 (22.2 with twice as many), 42 x 8192 x 2048 17.9 (21.8).
+  const int64_t most_blocks = steps <= 9 ? 128 : steps <= 32 ? 64 : 0;
+  int rows, room;
+  for (p.groups = (int)cdiv(M, SK_MAXROWS / P);; p.groups *= 2) {
+    p.mg = (int)cdiv(M, p.groups);
+    p.groups = (int)cdiv(M, p.mg);
+    rows = P * p.mg;
+    p.rt = (int)cdiv(rows, 16);
+    room = (int)((skinny_lds(p.rt) / rows - 16) / 256);  // steps whose image fits
+    p.wk = 1;
+    while (p.wk < SK_WAVES && 2 * p.wk <= steps && 2 * p.wk <= room && tiles * p.wk < 2048) p.wk *= 2;
+    p.gx = cdiv(tiles, SK_WAVES / p.wk);
+    if (p.rt == 1 || p.gx * p.groups > most_blocks) break;
+  }
   int64_t s = p.gx * p.groups < 256 ? cdiv(512, p.gx * p.groups) : 1;
   // a split costs a second launch (3 us): worth it down to four steps of each wave for one operand tile, to one for three or
   // four, whose steps take longer (16 x 1024 x 4096 transposed: 15.0 us at four, 11.2 at two, 9.5 at one; 1 x 4096 x 1024: 5.5, 6.7, 6.3)
@@ -44,6 +53,7 @@ static inline SkinnyPlan skinny_plan(int P, int64_t M, int64_t L, int64_t O) {
   if (s > most) s = most;
   if (s < 1) s = 1;
   if (s > 64) s = 64;
+  if (steps < 3 * p.wk) s = 1;  // less than three steps a wave are not worth a launch
   int64_t per = cdiv(steps, s);
   per = round_up(per, p.wk);
   p.splits = (int)cdiv(steps, per);
