@@ -5,6 +5,10 @@
 // vector instructions compete with the matrix ones) and staged through LDS, double buffered, 64 reduction indices at a time,
 // 16-byte chunks at chunk ^ (row / 2 % 8) so that fragment reads and stage writes are free of bank conflicts; the codes go
 // straight from memory to registers, one step ahead, and are decoded where they are used.
+// Measured, float32 (three pieces): 1024 x 4096 x 4096 96.5 us, 1068 TFLOP/s issued (a library product of two 8192 x 8192 bfloat16
+// matrices: 1213); matrix pipe busy 47 % of the cycles, other vector instructions 17 %.  1024 x 1024 x 4096 34.7 us of which 11
+// do not depend on the depth (launch, first loads, last stores) + 5.4 us for the planes; transposed 35.6 + 8.1 + 6.6 us for
+// the sum of four parts.
 #pragma once
 #include "frag.hpp"
 

@@ -917,7 +917,7 @@ def load_q8(q8, dtype=torch.float32):
 def dense_grads_q8(q8, dY, out=None):
     """(dW [K, N], db [N]) float32 of a dense layer y = x W + b from the 8-bit checkpoint of its input x [M, K] and
     dY [M, N] (float32, bfloat16 or float16): dW = x~^T dY, db = sum of dY's rows.  out: optional pair (dW, db) of float32
-    tensors to write to (db may be None: not wanted)."""
+    tensors to write to, not overlapping dY (db may be None: not wanted)."""
     M, K = q8.M, q8.K
     dY = _lb_mat("dense_grads_q8", "dY", dY, rows=M)
     dt, dev, N = _lb_dt("dense_grads_q8", dY), dY.get_device(), dY.shape[1]
@@ -934,6 +934,8 @@ def dense_grads_q8(q8, dY, out=None):
         if db is not None and (tuple(db.shape) != (N,) or db.dtype != torch.float32 or db.get_device() != dev
                                or not db.is_contiguous()):
             raise GpvaeError("dense_grads_q8: db must be contiguous float32 [%d] on %s" % (N, dY.device))
+        if M and dY.data_ptr() in (dW.data_ptr(), _ptr(db)):
+            raise GpvaeError("dense_grads_q8: out must not be dY")
     work = _lb_work("gpvae_dense_grads_q8_workspace_bytes", dt, M, K, N, dY)
     _lb_call("gpvae_dense_grads_q8", dev, _lib.load_lowbit().gpvae_dense_grads_q8, dt, M, K, N, 1 if q8.relu else 0,
              q8.codes.data_ptr(), q8.exps.data_ptr(), dY.data_ptr(), max(dY.stride(0), N), dW.data_ptr(), dW.stride(0), _ptr(db),

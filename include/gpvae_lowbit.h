@@ -17,6 +17,8 @@
  * after a ReLU; a tile of zeros has e = 0), but at most 125 (w4), 121 (q8), 120 (q8 after a ReLU): top * 2^e stays
  * finite, and only magnitudes above it (2.55e38 for w4, 3.38e38 for q8) saturate.  A tile that holds an infinity or a NaN gets the byte 255 and
  * reads as NaN throughout.  Every value the formats can hold is exactly a bfloat16 number.
+ * The products take a floating operand apart into bfloat16 pieces without rounding (three for float32, two for float16;
+ * bits below 2^-133, bfloat16's smallest, are dropped), so that only the float32 sums round.
  *
  *   w4   weights W [K, N] of a dense layer y = x W + b:  codes uint32 [ceil(K/32)][Np][4], Np = N rounded up to 32:
  *        nibble i (low first) of codes[kb][n][j] is row 32 kb + 8 j + i of column n — bit 3 the sign, bits 0-2 one of

@@ -333,6 +333,73 @@ def test_offsets_past_32_bits():
     close(dX[:, -64:], np64(dY) @ Wd.T, np.abs(np64(dY)) @ np.abs(Wd).T, N, F32)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,K,N", [(5, 256, 70), (20, 384, 200), (130, 128, 66), (300, 256, 258)])
+def test_alignment_changes_no_bit(M, K, N, dt):
+    """Whatever loads an operand's strides and alignment allow, the same sums in the same order."""
+    rng = np.random.default_rng(M + K + N)
+    w4, b = ops.quant_w4(normal(rng, (K, N), F32)), normal(rng, (N,), dt)
+    X, dY = normal(rng, (M, K), dt), normal(rng, (M, N), dt)
+    Y, q = ops.store_q8(X, relu=True)
+    Yd, dX, (dW, db) = ops.dense_w4(X, w4, b), ops.dense_vjp_w4(dY, w4, q), ops.dense_grads_q8(q, dY)
+    for lead, shift in [(0, 0), (3, 1), (2, 1), (8, 0), (6, 2), (5, 8), (64, 64)]:
+        vx, vy = strided(X, lead=lead, shift=shift)[1], strided(dY, lead=lead, shift=shift)[1]
+        Y2, q2 = ops.store_q8(vx, relu=True)
+        assert torch.equal(Y2, Y) and torch.equal(q2.codes, q.codes) and torch.equal(q2.exps, q.exps)
+        buf, out = strided(torch.zeros_like(Yd), lead=lead, shift=shift)
+        assert torch.equal(ops.dense_w4(vx, w4, b, out=out), Yd) and torch.equal(ops.dense_vjp_w4(vy, w4, q), dX)
+        assert (buf[M] == 7).all() and (buf[:, :shift] == 7).all() and (buf[:M, shift + N:] == 7).all()
+        wbuf, wout = strided(torch.zeros_like(dW), lead=lead, shift=shift)
+        got = ops.dense_grads_q8(q, vy, out=(wout, torch.empty_like(db)))
+        assert torch.equal(got[0], dW) and torch.equal(got[1], db)
+        assert (wbuf[K] == 7).all() and (wbuf[:, :shift] == 7).all() and (wbuf[:K, shift + N:] == 7).all()
+
+
+def test_gradients_are_not_written_over_their_input():
+    q = ops.store_q8(torch.ones((6, 6), device=DEV))
+    dY = torch.ones((6, 6), device=DEV)
+    for out in [(dY, None), (torch.empty((6, 6), device=DEV), dY[0])]:
+        with pytest.raises(GpvaeError):
+            ops.dense_grads_q8(q, dY, out=out)
+
+
+def test_operands_past_32_bits():
+    """Operands, their pieces, codes and outputs of more than 2^32 bytes: rows and columns at both ends."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(2)
+    M, K, N = 66000, 65600, 40
+    X = torch.randn((M, K), device=DEV, generator=g, dtype=BF16)
+    q = ops.store_q8(X)
+    assert q.codes.numel() > 2 ** 32
+    for rows in (slice(0, 16), slice(M - 16, M)):
+        mb = slice(rows.start // 8, rows.stop // 8)
+        cut = ops.store_q8(X[rows].contiguous())
+        assert torch.equal(q.codes[mb], cut.codes) and torch.equal(q.exps[mb], cut.exps)
+    dY = torch.randn((M, N), device=DEV, generator=g, dtype=BF16)
+    dW, db = ops.dense_grads_q8(q, dY)
+    for cols in (slice(0, 64), slice(K - 64, K)):
+        t = ops.load_q8(ops.Q8(q.codes[:, cols].contiguous(), q.exps[:, cols.start // 8:cols.stop // 8].contiguous(), M, 64)).double()
+        want, S = t.t() @ dY.double(), t.abs().t() @ dY.double().abs()
+        close(dW[cols], want.cpu().numpy(), S.cpu().numpy(), M, F32)
+    del q, dW
+    w4 = ops.quant_w4(torch.randn((K, N), device=DEV, generator=g))
+    Wd = ops.load_w4(w4).double()
+    rows = torch.cat([torch.arange(8), torch.arange(M - 8, M)]).to(DEV)
+    got = ops.dense_w4(X, w4)[rows]                                    # many rows, read in place
+    want, S = X[rows].double() @ Wd, X[rows].double().abs() @ Wd.abs()
+    close(got, want.cpu().numpy(), S.cpu().numpy(), K, BF16)
+    X = X[:24000].float()
+    rows = torch.cat([torch.arange(8), torch.arange(24000 - 8, 24000)]).to(DEV)
+    got = ops.dense_w4(X, w4)[rows]                                    # many rows, pieces of 9.4 GB
+    want, S = X[rows].double() @ Wd, X[rows].double().abs() @ Wd.abs()
+    close(got, want.cpu().numpy(), S.cpu().numpy(), K, F32)
+    wt = ops.quant_w4(Wd.t().contiguous().float())                     # [N, K]: its transposed product reduces over K
+    got = ops.dense_vjp_w4(X, wt)[rows]
+    Wt = ops.load_w4(wt).double()
+    want, S = X[rows].double() @ Wt.t(), X[rows].double().abs() @ Wt.abs().t()
+    close(got, want.cpu().numpy(), S.cpu().numpy(), K, F32)
+
+
 # ---- streams and graphs -------------------------------------------------------------------------------------------------
 def test_side_stream_and_replayed_graph():
     rng = np.random.default_rng(12)
