@@ -21,14 +21,15 @@ __global__ __launch_bounds__(256) void split_planes_kernel(int64_t M, int64_t L,
                                                            u32x2 *__restrict__ planes) {
   constexpr int P = Split<T>::P;
   const int64_t q = Lp / 4, m = ((int64_t)blockIdx.x << (8 - qsh)) + (threadIdx.x >> qsh);
-  const int64_t k4 = (int64_t)blockIdx.y * 256 + (threadIdx.x & ((1 << qsh) - 1));
-  if (m >= M || k4 >= q) return;
-  const Vec4<T> v = load4(X + m * ldx, k4 * 4, L);
-  uint32_t a[P], b[P];
-  Split<T>::two(v.v[0], v.v[1], a);
-  Split<T>::two(v.v[2], v.v[3], b);
+  if (m >= M) return;
+  for (int64_t k4 = (int64_t)blockIdx.y * 256 + (threadIdx.x & ((1 << qsh) - 1)); k4 < q; k4 += (int64_t)gridDim.y * 256) {
+    const Vec4<T> v = load4(X + m * ldx, k4 * 4, L);
+    uint32_t a[P], b[P];
+    Split<T>::two(v.v[0], v.v[1], a);
+    Split<T>::two(v.v[2], v.v[3], b);
 #pragma unroll
-  for (int p = 0; p < P; ++p) planes[p * M * q + ((k4 >> 4) * M + m) * 16 + (k4 & 15)] = u32x2{a[p], b[p]};
+    for (int p = 0; p < P; ++p) planes[p * M * q + ((k4 >> 4) * M + m) * 16 + (k4 & 15)] = u32x2{a[p], b[p]};
+  }
 }
 
 constexpr int TL_WM = 2, TL_MT = 2;  // TL_WM x 2 waves, each 16 TL_MT rows x 64 outputs
@@ -263,7 +264,7 @@ static void launch_tile(hipStream_t st, const TilePlan &p, int64_t M, int64_t L,
   if (!p.direct) {
     int qsh = 5;  // 2^qsh >= Lp / 4, at most 256 threads to a row
     while (qsh < 8 && (4 << qsh) < p.Lp) ++qsh;
-    hipLaunchKernelGGL((split_planes_kernel<T>), dim3((unsigned)cdiv(M, 256 >> qsh), (unsigned)cdiv(p.Lp, 1024)), dim3(256), 0, st,
+    hipLaunchKernelGGL((split_planes_kernel<T>), dim3((unsigned)cdiv(M, 256 >> qsh), (unsigned)(p.Lp < 1024 * 65535ll ? cdiv(p.Lp, 1024) : 65535)), dim3(256), 0, st,
                        M, L, p.Lp, qsh, X, ldx, (u32x2 *)work);
     planes = reinterpret_cast<const char *>(work);
     rs = 128, ss = M * 128, ps = M * p.Lp * 2;

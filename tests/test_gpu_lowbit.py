@@ -400,6 +400,19 @@ def test_operands_past_32_bits():
     close(got, want.cpu().numpy(), S.cpu().numpy(), K, F32)
 
 
+@pytest.mark.parametrize("M", [3, 22])
+def test_very_long_reductions(M):
+    """Small integers: the sums are exact."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(3)
+    K, N = 67200001, 8
+    w4 = ops.quant_w4(torch.randint(0, 2, (K, N), device=DEV, generator=g).mul_(2).sub_(1).to(BF16))
+    X = torch.randint(-1, 2, (M, K), device=DEV, generator=g, dtype=torch.int8).float()
+    want = sum(X[:, k:k + 2 ** 22].double() @ ops.load_w4(ops.W4(w4.codes[k // 32:(k + 2 ** 22) // 32].contiguous(), w4.exps[k // 32:(k + 2 ** 22) // 32].contiguous(), min(2 ** 22, K - k), N)).double()
+               for k in range(0, K, 2 ** 22))
+    assert torch.equal(ops.dense_w4(X, w4).double(), want)
+
+
 # ---- streams and graphs -------------------------------------------------------------------------------------------------
 def test_side_stream_and_replayed_graph():
     rng = np.random.default_rng(12)
