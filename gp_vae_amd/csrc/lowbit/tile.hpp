@@ -4,11 +4,12 @@
 // planes ONCE by split_planes_kernel (a workgroup splitting its own rows would repeat that for every 128 outputs, and
 // vector instructions compete with the matrix ones) and staged through LDS, double buffered, 64 reduction indices at a time,
 // 16-byte chunks at chunk ^ (row / 2 % 8) so that fragment reads and stage writes are free of bank conflicts; the codes go
-// straight from memory to registers, one step ahead, and are decoded where they are used.
-// Measured, float32 (three pieces): 1024 x 4096 x 4096 96.5 us, 1068 TFLOP/s issued (a library product of two 8192 x 8192 bfloat16
-// matrices: 1213); matrix pipe busy 47 % of the cycles, other vector instructions 17 %.  1024 x 1024 x 4096 34.7 us of which 11
-// do not depend on the depth (launch, first loads, last stores) + 5.4 us for the planes; transposed 35.6 + 8.1 + 6.6 us for
-// the sum of four parts.
+// straight from memory to registers, one step ahead, and are decoded a half step before they are used.
+// Measured, float32 (three pieces): 1024 x 4096 x 4096 89 us, 1160 TFLOP/s issued (a library product of two 8192 x 8192 bfloat16
+// matrices: 1213).  1024 x 1024 x 4096 34.6 us in all, of which 11 do not depend on the depth (launch, first loads, last
+// stores) and 5.5 are for the planes; transposed 49 us with 8.1 for the planes and 6.7 for the sum of four parts.  Before the
+// halves were interleaved (all reads, all decoding, all products, all writes): 104, 36.7 and 50.2 us.  Tiles of 128 rows
+// (wave tiles 64 x 64, one workgroup a unit): 125 and 41.
 #pragma once
 #include "frag.hpp"
 
@@ -93,11 +94,14 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
   // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
   // may not have been issued does not count, so that the wait would reach into the step just issued.  Past the last step
   // the last one is read again.
-  auto issue = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
+  auto issue_stage = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
     s = s < s_hi ? s : s_hi - 1;
     const char *const b = pbase + s * ss;
 #pragma unroll
     for (int i = 0; i < NLD; ++i) h.st[i] = *reinterpret_cast<const u32x4 *>(b + (i / NR) * ps + src[i % NR]);
+  };
+  auto issue_codes = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
+    s = s < s_hi ? s : s_hi - 1;
     const int64_t sc = s < s_codes ? s : s_codes;  // the planes may go on past the last step with codes
     if (!VJP) {
       const char *const cb = codes + 2 * sc * Np * 16, *const eb = exps + 2 * sc * (Np / 2);
@@ -131,60 +135,88 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
 #pragma unroll
     for (int b = 0; b < 4; ++b) acc[a][b] = f32x4_t{0, 0, 0, 0};
   const int arow = (wm * MT * 16 + l16) * 128, sw = l16 >> 1;
-  // one step: codes of step s in `now`, its stage in lds[b]; `next` holds step s + 1 in flight, step s + 2 replaces `now`
-  auto step = [&](Ahead &now, Ahead &next, int64_t s, int b) __attribute__((always_inline)) {
-    u32x2 w[4];
-    uint32_t e[4];
+  u32x4 x[2][P][MT], f[2][4];
+  auto read = [&](int t, int b) __attribute__((always_inline)) {
+    const int ck = ((t * 4 + c) ^ sw) * 16;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) w[t] = now.cw[t], e[t] = now.ce[t] >> (16 * (VJP ? half : c & 1));
-    u32x4 x[2][P][MT], f[2][4];
-    auto read = [&](int t) __attribute__((always_inline)) {
-      const int ck = ((t * 4 + c) ^ sw) * 16;
+    for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p)
+      for (int a = 0; a < MT; ++a) x[t][p][a] = *reinterpret_cast<const u32x4 *>(lds[b] + p * BM * 128 + arow + a * 2048 + ck);
+  };
+  auto decode = [&](const Ahead &h, int t) __attribute__((always_inline)) {
+    if (!VJP) {
 #pragma unroll
-        for (int a = 0; a < MT; ++a) x[t][p][a] = *reinterpret_cast<const u32x4 *>(lds[b] + p * BM * 128 + arow + a * 2048 + ck);
-    };
-    auto decode = [&](int t) __attribute__((always_inline)) {
-      if (!VJP) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[t][i] = w4_frag(t ? w[i].y : w[i].x, t ? w4_scale<1>(e[i]) : w4_scale<0>(e[i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          f[t][2 * i] = w4_frag(tr(w[2 * t + i].x), w4_scale<0>(e[2 * t + i]));
-          f[t][2 * i + 1] = w4_frag(tr(w[2 * t + i].y), w4_scale<1>(e[2 * t + i]));
-        }
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t e = h.ce[i] >> (16 * (c & 1));
+        f[t][i] = w4_frag(t ? h.cw[i].y : h.cw[i].x, t ? w4_scale<1>(e) : w4_scale<0>(e));
       }
-    };
-    auto multiply = [&](int t) __attribute__((always_inline)) {
+    } else {
 #pragma unroll
-      for (int p = P - 1; p >= 0; --p)
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t e = h.ce[2 * t + i] >> (16 * half);
+        f[t][2 * i] = w4_frag(tr(h.cw[2 * t + i].x), w4_scale<0>(e));
+        f[t][2 * i + 1] = w4_frag(tr(h.cw[2 * t + i].y), w4_scale<1>(e));
+      }
+    }
+  };
+  auto multiply = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int a = 0; a < MT; ++a)
+    for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[a][i] = mfma(x[t][p][a], f[t][i], acc[a][i]);
-    };
-    // The codes are decoded before the loads that replace them are issued (else those go to other registers and are copied, and
-    // waited for, at the end of the turn), and a half step's fragments are read before the other half is multiplied.
-    read(0);
-    decode(0);
-    decode(1);
+      for (int a = 0; a < MT; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[a][i] = mfma(x[t][p][a], f[t][i], acc[a][i]);
+  };
+  // One step, in two halves of 32 indices.  Its first half's fragments are in registers, its stage in lds[b], its codes in `now`;
+  // `next` holds step s + 1 in flight.  While a half is multiplied, the other's fragments are read and decoded and the next
+  // stage is written, instruction by instruction: matrix, vector and LDS instructions overlap only when they alternate.  What
+  // has been written and decoded is replaced: the stage by step s + 3's in `next`, the codes by step s + 2's in `now`.
+  auto step = [&](Ahead &now, Ahead &next, int64_t s, int b) __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
-    issue(now, s + 2);
-    read(1);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(0);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(1);
+    __builtin_amdgcn_s_setprio(1);  // the unit's other workgroup is kept in the opposite half: 2-4 % faster
+    read(1, b);
+    decode(now, 1);
     put(next, b ^ 1);
+    multiply(0);
+#pragma unroll
+    for (int g = 0; g < 2 * P; ++g) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // a fragment read
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);  // a stage write
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
     __syncthreads();
+    __builtin_amdgcn_sched_barrier(0);
+    read(0, b ^ 1);
+    decode(next, 0);
+    issue_stage(next, s + 3);
+    issue_codes(now, s + 2);
+    multiply(1);
+#pragma unroll
+    for (int g = 0; g < 2 * P; ++g) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, (2 * P + 8 + 2 * P - 1) / (2 * P), 0);  // loads
+      __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
   Ahead h0, h1;
-  issue(h0, s_lo);
-  issue(h1, s_lo + 1);
+  issue_stage(h0, s_lo);
+  issue_codes(h0, s_lo);
+  issue_stage(h1, s_lo + 1);
+  issue_codes(h1, s_lo + 1);
   put(h0, 0);
+  issue_stage(h0, s_lo + 2);
   __syncthreads();
+  read(0, 0);
+  decode(h0, 0);
   // an even number of steps: a loop that may leave after the first of two makes the compiler copy registers whose loads are in
   // flight, and wait for them
 #pragma unroll 1
