@@ -71,15 +71,16 @@ __device__ __forceinline__ rsrc_t buffer(const char *base, int bytes) {
 // 2 lane and 2 lane + 1 with one load for both.
 template <typename T, bool PAIR> struct RowsOf {
   uint32_t w[8][PAIR ? 1 : 2];
-  __device__ __forceinline__ void load(rsrc_t r, int i, int lane) {
+  // row i, whose columns lie o0 and o1 bytes from the base
+  __device__ __forceinline__ void load(rsrc_t r, int i, uint32_t o0, uint32_t o1) {
     if constexpr (PAIR) {
-      w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, 0, 0);
+      w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, o0, 0, 0);
     } else if constexpr (sizeof(T) == 4) {
-      w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4, 0, 0);
-      w[i][1] = __builtin_amdgcn_raw_buffer_load_b32(r, lane * 4 + 256, 0, 0);
+      w[i][0] = __builtin_amdgcn_raw_buffer_load_b32(r, o0, 0, 0);
+      w[i][1] = __builtin_amdgcn_raw_buffer_load_b32(r, o1, 0, 0);
     } else {
-      w[i][0] = __builtin_amdgcn_raw_buffer_load_b16(r, lane * 2, 0, 0);
-      w[i][1] = __builtin_amdgcn_raw_buffer_load_b16(r, lane * 2 + 128, 0, 0);
+      w[i][0] = __builtin_amdgcn_raw_buffer_load_b16(r, o0, 0, 0);
+      w[i][1] = __builtin_amdgcn_raw_buffer_load_b16(r, o1, 0, 0);
     }
   }
   __device__ __forceinline__ T value(int i, int e) const {
@@ -110,7 +111,6 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   const int64_t k0 = (int64_t)kt * 128, n0 = (int64_t)nt * 128;
   const int s_lo = (int)blockIdx.y * steps, s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
   const int64_t Kp = q8_kp(K);
-  const int mbs = (int)q8_mb(M);
   const bool sum_db = db != nullptr && kt == 0;
   dW += blockIdx.y * part_stride;
   if (db) db += blockIdx.y * part_stride;
@@ -127,23 +127,43 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
     uint32_t e[2];
   };
   // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
-  // may not have been issued does not count, so that the wait would reach into the step just issued.
-  const int64_t rb = lddy * (int64_t)sizeof(T);
-  const char *const ybase = reinterpret_cast<const char *>(dY + n0);
+  // may not have been issued does not count, so that the wait would reach into the step just issued.  The steps are loaded in order:
+  // the bases move on by themselves, and the loop spends few scalar instructions on addresses (a wave issues one instruction in
+  // four cycles, and two waves share a SIMD).
+  const uint32_t rb = (uint32_t)(lddy * (int64_t)sizeof(T));
   const int ybytes = (int)(N - n0 < 128 ? N - n0 : 128) * (int)sizeof(T), xcols = (int)(Kp - k0 < 128 ? Kp - k0 : 128);
-  auto issue = [&](Ahead &h, int s) __attribute__((always_inline)) {
-    const int m = s * GR_ROWS + wave * 8, rows = s < s_hi ? (int)M - m : 0;
-    const char *const r = ybase + m * rb;
+  // columns past the last: the last one (pair) again, results unused
+  const int yl0 = ycol0 * (int)sizeof(T), yl1 = ycol1 * (int)sizeof(T), ylast = ybytes - (PAIR ? 2 : 1) * (int)sizeof(T);
+  uint32_t yo[8][2];  // lddy <= 2^26: 8 rows lie within a 32-bit offset (the scalar offset is not part of the range check)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h.y.load(buffer(r + i * rb, i < rows ? ybytes : 0), i, lane);
+  for (int i = 0; i < 8; ++i) yo[i][0] = (uint32_t)i * rb + (yl0 < ylast ? yl0 : ylast), yo[i][1] = (uint32_t)i * rb + (yl1 < ylast ? yl1 : ylast);
+  int64_t m_end = (int64_t)s_hi * GR_ROWS;
+  m_end = m_end < M ? m_end : M;
+  int left = (int)(m_end - (int64_t)s_lo * GR_ROWS);  // rows from the next step's first to the last of this workgroup
+  const char *yb = reinterpret_cast<const char *>(dY + n0) + ((int64_t)s_lo * GR_ROWS + wave * 8) * (int64_t)rb;
+  const char *qb[2], *eb[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t at = ((int64_t)s_lo * (GR_ROWS / 8) + xb + 4 * j) * Kp + k0;
+    qb[j] = codes + at * 8;
+    eb[j] = exps + at / 8;
+  }
+  auto issue = [&](Ahead &h) __attribute__((always_inline)) {
+    int rows = left - wave * 8;
+    rows = rows < 8 ? rows : 8;
+    const rsrc_t ry = buffer(yb, rows > 0 ? (int)((rows - 1) * rb + ybytes) : 0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h.y.load(ry, i, yo[i][0], yo[i][1]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int mb = s * (GR_ROWS / 8) + xb + 4 * j;
-      const bool in = s < s_hi && mb < mbs;
-      const int64_t at = mb * Kp + k0;
-      h.q[j] = __builtin_amdgcn_raw_buffer_load_b64(buffer(codes + at * 8, in ? xcols * 8 : 0), xk * 8, 0, 0);
-      h.e[j] = __builtin_amdgcn_raw_buffer_load_b8(buffer(exps + at / 8, in ? xcols / 8 : 0), xk / 8, 0, 0);
+      const bool in = left > (xb + 4 * j) * 8;
+      h.q[j] = __builtin_amdgcn_raw_buffer_load_b64(buffer(qb[j], in ? xcols * 8 : 0), xk * 8, 0, 0);
+      h.e[j] = __builtin_amdgcn_raw_buffer_load_b8(buffer(eb[j], in ? xcols / 8 : 0), xk / 8, 0, 0);
+      qb[j] += Kp * (GR_ROWS / 8 * 8);
+      eb[j] += Kp;
     }
+    yb += (int64_t)rb * GR_ROWS;
+    left -= GR_ROWS;
   };
   float dbacc[2] = {0.0f, 0.0f};
   auto put = [&](const Ahead &h, int b) __attribute__((always_inline)) {
@@ -195,16 +215,16 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
           for (int i = 0; i < 2; ++i) acc[a][i] = mfma(x[t][a], y[t][p][i], acc[a][i]);
   };
   // Step s is in lds[b], `next` holds s + 1 in flight, s + 2 replaces `now`.
-  auto step = [&](Ahead &now, Ahead &next, int s, int b) __attribute__((always_inline)) {
-    issue(now, s + 2);
+  auto step = [&](Ahead &now, Ahead &next, int b) __attribute__((always_inline)) {
+    issue(now);
     multiply(b);
     put(next, b ^ 1);
     __syncthreads();
   };
   Ahead h0, h1;
   if (s_lo < s_hi) {
-    issue(h0, s_lo);
-    issue(h1, s_lo + 1);
+    issue(h0);
+    issue(h1);
     put(h0, 0);
   }
   __syncthreads();
@@ -212,8 +232,8 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   // compiler copy registers whose loads are in flight, and wait for them
 #pragma unroll 1
   for (int s = s_lo; s < s_hi; s += 2) {
-    step(h0, h1, s, 0);
-    step(h1, h0, s + 1, 1);
+    step(h0, h1, 0);
+    step(h1, h0, 1);
   }
 #pragma unroll
   for (int a = 0; a < 4; ++a)

@@ -186,11 +186,13 @@ extern "C" int gpvae_dense_grads_q8(void *stream, int dtype, int64_t M, int64_t 
                                     void *work) {
   const char *fn = "gpvae_dense_grads_q8";
   if (const int rc = check_q8(fn, dtype, M, K)) return rc;
-  LB_REQUIRE(N >= 1 && N <= (1 << 30), 5, "%s: N must lie in [1, 2^30] (got %lld)", fn, (long long)N);
+  LB_REQUIRE(N >= 1 && N <= (1 << 26), 5, "%s: N must lie in [1, 2^26] (got %lld)", fn, (long long)N);
   LB_REQUIRE(M == 0 || (codes && aligned16(codes)), 7, "%s: codes must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(M == 0 || (exps && aligned16(exps)), 8, "%s: exps must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(M == 0 || dY, 9, "%s: dY is NULL", fn);
   LB_REQUIRE(M == 0 || lddy >= N, 10, "%s: lddy < N", fn);
+  if (M <= 1) lddy = N;
+  LB_REQUIRE(lddy <= (1 << 26), 10, "%s: lddy must not exceed 2^26 (got %lld)", fn, (long long)lddy);
   LB_REQUIRE(dW, 11, "%s: dW is NULL", fn);
   LB_REQUIRE(lddw >= N, 12, "%s: lddw < N", fn);
   LB_REQUIRE(!gpvae_dense_grads_q8_workspace_bytes(dtype, M, K, N) || (work && aligned16(work)), 14,
