@@ -119,8 +119,10 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   // + 4.  Everything outside the matrices, and a step past the last, is loaded as zero.
   const int xk = tid & 127, xb = wave >> 1;
   const int ycol0 = PAIR ? 2 * lane : lane, ycol1 = PAIR ? ycol0 + 1 : lane + 64;
-  const int ydst0 = AB + ycol0 * 128 + ((wave ^ ((ycol0 >> 1) & 7)) * 16), ydst1 = ydst0 + (ycol1 - ycol0) * 128;  // same swizzle
-  const int xsw = (xk >> 1) & 7;
+  // 16-byte chunks of an image row at chunk ^ (row % 8), or, where a thread writes two neighbouring rows, chunk ^ (row / 2 % 8): eight
+  // consecutive lanes then write to, and a fragment's lanes read from, different banks
+  const int ydst0 = AB + ycol0 * 128 + ((wave ^ ((PAIR ? ycol0 >> 1 : ycol0) & 7)) * 16), ydst1 = ydst0 + (ycol1 - ycol0) * 128;
+  const int xsw = xk & 7;
   struct Ahead {
     RowsOf<T, PAIR> y;
     u32x2 q[2];
@@ -192,18 +194,18 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int i = 0; i < 2; ++i) acc[a][i] = f32x4_t{0, 0, 0, 0};
-  const int arow = (wk * 64 + l16) * 128, brow = AB + (wn * 32 + l16) * 128, sw = l16 >> 1;
+  const int arow = (wk * 64 + l16) * 128, brow = AB + (wn * 32 + l16) * 128, xrsw = l16 & 7, yrsw = PAIR ? l16 >> 1 : l16 & 7;
   auto multiply = [&](int b) __attribute__((always_inline)) {
     u32x4 x[2][4], y[2][P][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int ck = ((t * 4 + c) ^ sw) * 16;
+      const int xc = ((t * 4 + c) ^ xrsw) * 16, yc = ((t * 4 + c) ^ yrsw) * 16;
 #pragma unroll
-      for (int a = 0; a < 4; ++a) x[t][a] = *reinterpret_cast<const u32x4 *>(lds[b] + arow + a * 2048 + ck);
+      for (int a = 0; a < 4; ++a) x[t][a] = *reinterpret_cast<const u32x4 *>(lds[b] + arow + a * 2048 + xc);
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) y[t][p][i] = *reinterpret_cast<const u32x4 *>(lds[b] + brow + p * AB + i * 2048 + ck);
+        for (int i = 0; i < 2; ++i) y[t][p][i] = *reinterpret_cast<const u32x4 *>(lds[b] + brow + p * AB + i * 2048 + yc);
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t)
