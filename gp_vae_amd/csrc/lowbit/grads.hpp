@@ -115,18 +115,17 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   dW += blockIdx.y * part_stride;
   if (db) db += blockIdx.y * part_stride;
 
-  // dY share: two columns, rows 8 wave .. + 7 of the step; checkpoint share: column tid % 128, blocks of 8 rows tid / 128 and
-  // + 4.  Everything outside the matrices, and a step past the last, is loaded as zero.
-  const int xk = tid & 127, xb = wave >> 1;
+  // dY share: two columns, rows 8 wave .. + 7 of the step; checkpoint share: columns 2 lane and 2 lane + 1 of the same rows,
+  // which are one tile row.  Everything outside the matrices, and a step past the last, is loaded as zero.
   const int ycol0 = PAIR ? 2 * lane : lane, ycol1 = PAIR ? ycol0 + 1 : lane + 64;
-  // 16-byte chunks of an image row at chunk ^ (row % 8), or, where a thread writes two neighbouring rows, chunk ^ (row / 2 % 8): eight
-  // consecutive lanes then write to, and a fragment's lanes read from, different banks
-  const int ydst0 = AB + ycol0 * 128 + ((wave ^ ((PAIR ? ycol0 >> 1 : ycol0) & 7)) * 16), ydst1 = ydst0 + (ycol1 - ycol0) * 128;
-  const int xsw = xk & 7;
+  // 16-byte chunks of an image row at chunk ^ (row / 2 % 8) where a thread writes two neighbouring rows, at chunk ^ (row % 8) where
+  // neighbouring threads do: eight consecutive lanes then write to, and a fragment's lanes read from, different banks
+  const int ydst0 = AB + ycol0 * 128 + ((wave ^ ((PAIR ? lane : ycol0) & 7)) * 16), ydst1 = ydst0 + (ycol1 - ycol0) * 128;
+  const int xdst = lane * 256 + ((wave ^ (lane & 7)) * 16);
   struct Ahead {
     RowsOf<T, PAIR> y;
-    u32x2 q[2];
-    uint32_t e[2];
+    u32x4 q;
+    uint32_t e;
   };
   // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
   // may not have been issued does not count, so that the wait would reach into the step just issued.  The steps are loaded in order:
@@ -143,27 +142,18 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   m_end = m_end < M ? m_end : M;
   int left = (int)(m_end - (int64_t)s_lo * GR_ROWS);  // rows from the next step's first to the last of this workgroup
   const char *yb = reinterpret_cast<const char *>(dY + n0) + ((int64_t)s_lo * GR_ROWS + wave * 8) * (int64_t)rb;
-  const char *qb[2], *eb[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t at = ((int64_t)s_lo * (GR_ROWS / 8) + xb + 4 * j) * Kp + k0;
-    qb[j] = codes + at * 8;
-    eb[j] = exps + at / 8;
-  }
+  const int64_t at = ((int64_t)s_lo * (GR_ROWS / 8) + wave) * Kp + k0;
+  const char *qb = codes + at * 8, *eb = exps + at / 8;
   auto issue = [&](Ahead &h) __attribute__((always_inline)) {
     int rows = left - wave * 8;
     rows = rows < 8 ? rows : 8;
     const rsrc_t ry = buffer(yb, rows > 0 ? (int)((rows - 1) * rb + ybytes) : 0);
 #pragma unroll
     for (int i = 0; i < 8; ++i) h.y.load(ry, i, yo[i][0], yo[i][1]);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const bool in = left > (xb + 4 * j) * 8;
-      h.q[j] = __builtin_amdgcn_raw_buffer_load_b64(buffer(qb[j], in ? xcols * 8 : 0), xk * 8, 0, 0);
-      h.e[j] = __builtin_amdgcn_raw_buffer_load_b8(buffer(eb[j], in ? xcols / 8 : 0), xk / 8, 0, 0);
-      qb[j] += Kp * (GR_ROWS / 8 * 8);
-      eb[j] += Kp;
-    }
+    h.q = __builtin_amdgcn_raw_buffer_load_b128(buffer(qb, rows > 0 ? xcols * 8 : 0), lane * 16, 0, 0);
+    h.e = __builtin_amdgcn_raw_buffer_load_b8(buffer(eb, rows > 0 ? xcols / 8 : 0), lane / 4, 0, 0);
+    qb += Kp * GR_ROWS;
+    eb += Kp;
     yb += (int64_t)rb * GR_ROWS;
     left -= GR_ROWS;
   };
@@ -178,9 +168,8 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
       for (int p = 0; p < P; ++p)
         *reinterpret_cast<u32x4 *>(lds[b] + (e ? ydst1 : ydst0) + p * AB) = u32x4{w[0][p], w[1][p], w[2][p], w[3][p]};
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      *reinterpret_cast<u32x4 *>(lds[b] + xk * 128 + (((xb + 4 * j) ^ xsw) * 16)) = q8_frag<RELU>(h.q[j], h.e[j]);
+    *reinterpret_cast<u32x4 *>(lds[b] + xdst) = q8_frag<RELU>(u32x2{h.q.x, h.q.y}, h.e);
+    *reinterpret_cast<u32x4 *>(lds[b] + xdst + 128) = q8_frag<RELU>(u32x2{h.q.z, h.q.w}, h.e);
     if (sum_db) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
@@ -194,7 +183,7 @@ __global__ __launch_bounds__(GR_THREADS, 2) void grads_kernel(int64_t M, int64_t
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int i = 0; i < 2; ++i) acc[a][i] = f32x4_t{0, 0, 0, 0};
-  const int arow = (wk * 64 + l16) * 128, brow = AB + (wn * 32 + l16) * 128, xrsw = l16 & 7, yrsw = PAIR ? l16 >> 1 : l16 & 7;
+  const int arow = (wk * 64 + l16) * 128, brow = AB + (wn * 32 + l16) * 128, xrsw = l16 >> 1, yrsw = PAIR ? l16 >> 1 : l16 & 7;
   auto multiply = [&](int b) __attribute__((always_inline)) {
     u32x4 x[2][4], y[2][P][2];
 #pragma unroll
