@@ -20,6 +20,12 @@ __device__ __forceinline__ int64_t xcd_chunk(int64_t id, int64_t n) {
   return x * q + (x < r ? x : r) + (id >> 3);
 }
 
+// A buffer of `bytes` at a wave-uniform base: what lies past it reads as zero, without an access.
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t buffer(const char *base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, bytes, 0x00027000);
+}
+
 // ---- w4 -----------------------------------------------------------------------------------------------------------------
 // 8 codes -> 8 bfloat16 values; byte J of the tile-exponent word e is their exponent.  The conversion uses the scale's exponent
 // bits alone (checked over all exponents with random sign and mantissa bits): the neighbouring bytes need no masking.

@@ -61,12 +61,6 @@ template <bool RELU> __device__ __forceinline__ u32x4 q8_frag(u32x2 q, uint32_t 
   return u32x4{pack_hi(v[0], v[1]), pack_hi(v[2], v[3]), pack_hi(v[4], v[5]), pack_hi(v[6], v[7])};
 }
 
-// A buffer of `bytes` at a wave-uniform base: what lies past it reads as zero, without an access.
-typedef __amdgpu_buffer_rsrc_t rsrc_t;
-__device__ __forceinline__ rsrc_t buffer(const char *base, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(base), 0, bytes, 0x00027000);
-}
-
 // What a thread has loaded of dY for a step: 8 rows of two columns, which are lane and lane + 64, or, for two-byte types (PAIR),
 // 2 lane and 2 lane + 1 with one load for both.
 template <typename T, bool PAIR> struct RowsOf {

@@ -49,7 +49,8 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
   __shared__ __align__(16) unsigned char lds[2][CH * 16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wo = wave & 1, c = lane >> 4, l16 = lane & 15;
-  const int64_t bt = blockIdx.x, m0 = (bt % mtiles) * BM, o0 = (bt / mtiles) * 128 + wo * 64;  // row tiles fastest
+  const uint32_t ot = __builtin_amdgcn_readfirstlane(blockIdx.x / (uint32_t)mtiles);  // row tiles fastest
+  const int64_t m0 = (int64_t)(blockIdx.x - ot * (uint32_t)mtiles) * BM, o0 = (int64_t)ot * 128 + wo * 64;
   const int64_t s_lo = (int64_t)blockIdx.y * steps, s_hi = s_lo + steps < s_all ? s_lo + steps : s_all;
   Tr8 tr;
   if (VJP) tr.init(lane);
@@ -64,14 +65,13 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
     const int64_t row = trow + i * RP;
     src[i] = (uint32_t)((m0 + row < M ? row : M - 1 - m0) * rs) + ck8 * 16;  // rows past the last: results unused
   }
-  const char *const pbase = planes + m0 * rs;
   // lane group c reads chunk 2 c + t (product) or 4 t + c: either is kept at 4 t + c, so that the reads of the lane groups that
   // share a cycle never meet in a bank
   const int pk8 = VJP ? ck8 : (ck8 >> 1) | (ck8 & 1) << 2;
   const int dst = (trow * 8 + (pk8 ^ ((trow >> 1) & 7))) * 16;
-  // codes of one step: product: 8 bytes (two groups of 8 rows) of each of 4 columns 16 apart, lane group c taking rows
+  // Codes of one step: product: 8 bytes (two groups of 8 rows) of each of 4 columns 16 apart, lane group c taking rows
   // 32 (c / 2) + 16 (c % 2) + ...; transposed product: 8 bytes of a column for two blocks of 32 columns x two of 32 rows.
-  // Past the ends the last codes are read again: their outputs are unused, or they meet the operand's zeros.
+  // What lies past the last block is loaded as zero; columns (rows) past the last repeat the last one or its block, unused.
   uint32_t coff[4], eoff[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
@@ -84,44 +84,47 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
       eoff[t] = ((t >> 1) * 4 + c) * 4;
     }
   }
-  const int64_t kbv0 = VJP ? (o0 / 32 < kbs ? o0 / 32 : kbs - 1) : 0, kbv1 = VJP ? (o0 / 32 + 1 < kbs ? o0 / 32 + 1 : kbs - 1) : 0;
-  const int64_t s_codes = VJP ? (Np - 1) / 64 : (kbs - 1) / 2;
   struct Ahead {  // what is in flight for a step: its share of the stage, its codes and tile exponents
     u32x4 st[NLD];
     u32x2 cw[4];
     uint32_t ce[4];
   };
   // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
-  // may not have been issued does not count, so that the wait would reach into the step just issued.  Past the last step
-  // the last one is read again.
-  auto issue_stage = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
-    s = s < s_hi ? s : s_hi - 1;
-    const char *const b = pbase + s * ss;
+  // may not have been issued does not count, so that the wait would reach into the step just issued.  The steps are loaded in
+  // order, each by scalar bases that move on by themselves; past the last one nothing is read.
+  const char *pb = planes + m0 * rs + s_lo * ss;
+  int stages = (int)(s_all - s_lo);  // steps from here to the planes' end
+  auto issue_stage = [&](Ahead &h) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NLD; ++i) h.st[i] = *reinterpret_cast<const u32x4 *>(b + (i / NR) * ps + src[i % NR]);
+    for (int i = 0; i < NLD; ++i)
+      h.st[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer(pb + (i / NR) * ps, stages > 0 ? 0x7fffffff : 0), src[i % NR], 0, 0);
+    pb += ss;
+    --stages;
   };
-  auto issue_codes = [&](Ahead &h, int64_t s) __attribute__((always_inline)) {
-    s = s < s_hi ? s : s_hi - 1;
-    const int64_t sc = s < s_codes ? s : s_codes;  // the planes may go on past the last step with codes
+  const int64_t kbv0 = o0 / 32 < kbs ? o0 / 32 : kbs - 1, kbv1 = o0 / 32 + 1 < kbs ? o0 / 32 + 1 : kbs - 1;
+  const int64_t cat0 = VJP ? kbv0 * Np + s_lo * 64 : 2 * s_lo * Np, cat1 = kbv1 * Np + s_lo * 64;
+  const char *cb0 = codes + cat0 * 16, *cb1 = codes + cat1 * 16, *eb0 = exps + cat0 / 2, *eb1 = exps + cat1 / 2;
+  int64_t ends = VJP ? Np - s_lo * 64 : kbs - 2 * s_lo;  // columns (blocks of 32 rows) from here to the codes' end
+  auto issue_codes = [&](Ahead &h) __attribute__((always_inline)) {
     if (!VJP) {
-      const char *const cb = codes + 2 * sc * Np * 16, *const eb = exps + 2 * sc * (Np / 2);
-      const bool odd = 2 * sc + 1 >= kbs;  // the last block has no second one: lane groups 2, 3 read the first again
-      const uint32_t back_c = odd && c >= 2 ? (uint32_t)(Np * 16) : 0u, back_e = odd && c >= 2 ? (uint32_t)(Np / 2) : 0u;
+      const int nb = ends >= 2 ? 2 : ends == 1 ? 1 : 0;
+      const rsrc_t rc = buffer(cb0, nb * (int)Np * 16), re = buffer(eb0, nb * (int)Np / 2);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        h.cw[t] = *reinterpret_cast<const u32x2 *>(cb + (coff[t] - back_c));
-        h.ce[t] = *reinterpret_cast<const uint32_t *>(eb + (eoff[t] - back_e));
+        h.cw[t] = __builtin_amdgcn_raw_buffer_load_b64(rc, coff[t], 0, 0);
+        h.ce[t] = __builtin_amdgcn_raw_buffer_load_b32(re, eoff[t], 0, 0);
       }
+      cb0 += Np * 32, eb0 += Np;
+      ends -= 2;
     } else {
-      // columns 64 s + 32 (t / 2) ...: a second half past the end repeats the first
-      const uint32_t back = sc * 64 + 32 >= Np ? 32u : 0u;
+      const int nc = ends >= 64 ? 64 : ends > 0 ? (int)ends : 0;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int64_t kb = t & 1 ? kbv1 : kbv0;
-        const uint32_t bk = t >> 1 ? back : 0u;
-        h.cw[t] = *reinterpret_cast<const u32x2 *>(codes + (kb * Np + sc * 64) * 16 + (coff[t] - bk * 16));
-        h.ce[t] = *reinterpret_cast<const uint32_t *>(exps + (kb * Np + sc * 64) / 2 + (eoff[t] - bk / 2));
+        h.cw[t] = __builtin_amdgcn_raw_buffer_load_b64(buffer(t & 1 ? cb1 : cb0, nc * 16), coff[t], 0, 0);
+        h.ce[t] = __builtin_amdgcn_raw_buffer_load_b32(buffer(t & 1 ? eb1 : eb0, nc / 2), eoff[t], 0, 0);
       }
+      cb0 += 1024, cb1 += 1024, eb0 += 32, eb1 += 32;
+      ends -= 64;
     }
   };
   auto put = [&](const Ahead &h, int b) __attribute__((always_inline)) {
@@ -171,7 +174,7 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
   // `next` holds step s + 1 in flight.  While a half is multiplied, the other's fragments are read and decoded and the next
   // stage is written, instruction by instruction: matrix, vector and LDS instructions overlap only when they alternate.  What
   // has been written and decoded is replaced: the stage by step s + 3's in `next`, the codes by step s + 2's in `now`.
-  auto step = [&](Ahead &now, Ahead &next, int64_t s, int b) __attribute__((always_inline)) {
+  auto step = [&](Ahead &now, Ahead &next, int b) __attribute__((always_inline)) {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_setprio(1);  // the unit's other workgroup is kept in the opposite half: 2-4 % faster
     read(1, b);
@@ -193,8 +196,8 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
     __builtin_amdgcn_sched_barrier(0);
     read(0, b ^ 1);
     decode(next, 0);
-    issue_stage(next, s + 3);
-    issue_codes(now, s + 2);
+    issue_stage(next);
+    issue_codes(now);
     multiply(1);
 #pragma unroll
     for (int g = 0; g < 2 * P; ++g) {
@@ -208,12 +211,12 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
     __builtin_amdgcn_sched_barrier(0);
   };
   Ahead h0, h1;
-  issue_stage(h0, s_lo);
-  issue_codes(h0, s_lo);
-  issue_stage(h1, s_lo + 1);
-  issue_codes(h1, s_lo + 1);
+  issue_stage(h0);
+  issue_codes(h0);
+  issue_stage(h1);
+  issue_codes(h1);
   put(h0, 0);
-  issue_stage(h0, s_lo + 2);
+  issue_stage(h0);
   __syncthreads();
   read(0, 0);
   decode(h0, 0);
@@ -221,8 +224,8 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
   // flight, and wait for them
 #pragma unroll 1
   for (int64_t s = s_lo; s < s_hi; s += 2) {
-    step(h0, h1, s, 0);
-    step(h1, h0, s + 1, 1);
+    step(h0, h1, 0);
+    step(h1, h0, 1);
   }
   const bool whole = gridDim.y == 1;
   int64_t oi[4];
