@@ -78,16 +78,16 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
     if (!VJP) {
       const int64_t n = o0 + t * 16 + l16 < Np ? o0 + t * 16 + l16 : Np - 1;
       coff[t] = (uint32_t)(((c >> 1) * Np + n) * 16 + (c & 1) * 8);
-      eoff[t] = (uint32_t)(((c >> 1) * (Np / 8) + n / 8) * 4);
+      eoff[t] = (uint32_t)(((c >> 1) * (Np / 8) + n / 8) * 4 + 2 * (c & 1));
     } else {
       coff[t] = ((t >> 1) * 32 + c * 8 + lab) * 16 + half * 8;
-      eoff[t] = ((t >> 1) * 4 + c) * 4;
+      eoff[t] = ((t >> 1) * 4 + c) * 4 + 2 * half;
     }
   }
   struct Ahead {  // what is in flight for a step: its share of the stage, its codes and tile exponents
     u32x4 st[NLD];
     u32x2 cw[4];
-    uint32_t ce[4];
+    uint32_t ce[4];  // the exponents of both halves' tiles
   };
   // No branch may surround these loads: the wait for a step's loads counts the younger ones behind them, and a load that
   // may not have been issued does not count, so that the wait would reach into the step just issued.  The steps are loaded in
@@ -104,24 +104,24 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
   const int64_t kbv0 = o0 / 32 < kbs ? o0 / 32 : kbs - 1, kbv1 = o0 / 32 + 1 < kbs ? o0 / 32 + 1 : kbs - 1;
   const int64_t cat0 = VJP ? kbv0 * Np + s_lo * 64 : 2 * s_lo * Np, cat1 = kbv1 * Np + s_lo * 64;
   const char *cb0 = codes + cat0 * 16, *cb1 = codes + cat1 * 16, *eb0 = exps + cat0 / 2, *eb1 = exps + cat1 / 2;
-  int64_t ends = VJP ? Np - s_lo * 64 : kbs - 2 * s_lo;  // columns (blocks of 32 rows) from here to the codes' end
+  int ends = (int)(VJP ? Np - s_lo * 64 : kbs - 2 * s_lo);  // columns (blocks of 32 rows) from here to the codes' end
   auto issue_codes = [&](Ahead &h) __attribute__((always_inline)) {
     if (!VJP) {
-      const int nb = ends >= 2 ? 2 : ends == 1 ? 1 : 0;
-      const rsrc_t rc = buffer(cb0, nb * (int)Np * 16), re = buffer(eb0, nb * (int)Np / 2);
+      const int bytes = ends >= 2 ? (int)Np : ends == 1 ? (int)Np / 2 : 0;  // of exponents; 32 times as many of codes
+      const rsrc_t rc = buffer(cb0, bytes * 32), re = buffer(eb0, bytes);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         h.cw[t] = __builtin_amdgcn_raw_buffer_load_b64(rc, coff[t], 0, 0);
-        h.ce[t] = __builtin_amdgcn_raw_buffer_load_b32(re, eoff[t], 0, 0);
+        h.ce[t] = __builtin_amdgcn_raw_buffer_load_b16(re, eoff[t], 0, 0);
       }
       cb0 += Np * 32, eb0 += Np;
       ends -= 2;
     } else {
-      const int nc = ends >= 64 ? 64 : ends > 0 ? (int)ends : 0;
+      const int nc = __builtin_amdgcn_readfirstlane(ends >= 64 ? 64 : ends > 0 ? ends : 0);  // (a vector instruction clamps)
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         h.cw[t] = __builtin_amdgcn_raw_buffer_load_b64(buffer(t & 1 ? cb1 : cb0, nc * 16), coff[t], 0, 0);
-        h.ce[t] = __builtin_amdgcn_raw_buffer_load_b32(buffer(t & 1 ? eb1 : eb0, nc / 2), eoff[t], 0, 0);
+        h.ce[t] = __builtin_amdgcn_raw_buffer_load_b16(buffer(t & 1 ? eb1 : eb0, nc / 2), eoff[t], 0, 0);
       }
       cb0 += 1024, cb1 += 1024, eb0 += 32, eb1 += 32;
       ends -= 64;
@@ -150,13 +150,13 @@ __global__ __launch_bounds__(128 * TL_WM, 2) void tile_kernel(int64_t M, int64_t
     if (!VJP) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t e = h.ce[i] >> (16 * (c & 1));
+        const uint32_t e = h.ce[i];
         f[t][i] = w4_frag(t ? h.cw[i].y : h.cw[i].x, t ? w4_scale<1>(e) : w4_scale<0>(e));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint32_t e = h.ce[2 * t + i] >> (16 * half);
+        const uint32_t e = h.ce[2 * t + i];
         f[t][2 * i] = w4_frag(tr(h.cw[2 * t + i].x), w4_scale<0>(e));
         f[t][2 * i + 1] = w4_frag(tr(h.cw[2 * t + i].y), w4_scale<1>(e));
       }
