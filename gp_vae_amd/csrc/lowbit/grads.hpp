@@ -22,7 +22,7 @@ struct GradsPlan {
   int ktiles, splits, steps;
   int64_t blocks;
 };
-// Into how many parts are the rows split?  A step takes 0.5 + 0.37 P us (P pieces of dY), every full round of 256 workgroups
+// Into how many parts are the rows split?  A step takes 0.35 + 0.38 P us (P pieces of dY), every full round of 256 workgroups
 // anew; a split costs the launch that adds the parts (4 us) and writing and reading them.  The least of that estimate over
 // powers of two and the number that gives every unit a workgroup.  Measured, one part / two: bfloat16 300 x 700 x 1001
 // 10.8 / 15.8 us, float32 300 x 700 x 1000 14.3 / 18.3.
@@ -38,7 +38,7 @@ static inline GradsPlan grads_plan(int P, int64_t M, int64_t K, int64_t N) {
     for (int64_t s : {i, i < 256 ? int64_t(0) : 256 / p.blocks}) {
       if (s < 1 || (s > 1 && (s * p.blocks > 320 || s * 2 > steps))) continue;
       const int64_t per = round_up(cdiv(steps, s), 2), parts = cdiv(steps, per);
-      const double t = (double)(per * cdiv(parts * p.blocks, 256)) * (0.5 + 0.37 * P) +
+      const double t = (double)(per * cdiv(parts * p.blocks, 256)) * (0.35 + 0.38 * P) +
                        (parts > 1 ? 4.0 + (double)parts * ((double)(K + 1) * (double)N * (8 / 4.5e6) + 0.06) : 0.0);
       if (s == 1 || t < best) best = t, p.splits = (int)parts, p.steps = (int)per;
     }

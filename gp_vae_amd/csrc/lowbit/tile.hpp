@@ -263,8 +263,8 @@ struct TilePlan {
   bool direct;         // the operand itself is its only plane
 };
 
-// Into how many parts is the reduction split?  A step of 64 takes 0.27 + 0.24 P us where a compute unit has one workgroup and
-// 0.23 + 0.35 P us where it has the two that fit, every full round of 512 workgroups anew; a split costs the launch that adds
+// Into how many parts is the reduction split?  A step of 64 takes 0.25 + 0.22 P us where a compute unit has one workgroup and
+// 0.20 + 0.31 P us where it has the two that fit, every full round of 512 workgroups anew; a split costs the launch that adds
 // the parts (4 us) and writing and reading them.  The least of that estimate over powers of two and the numbers that give
 // every unit one or two workgroups.  Measured, one part / two / four: float32 512 x 4096 x 4096 78 / 65 us, 512 x 1024 x 4096
 // 28.2 / 33.5; float32 1024 x 1024 x 4096 transposed - / 59 / 51; bfloat16 1024 x 1000 x 1000 17.2 / 22.1.
@@ -282,7 +282,7 @@ static inline TilePlan tile_plan(int P, int64_t M, int64_t L, int64_t O, bool di
     for (int64_t s : {i, i < 256 ? int64_t(0) : 256 * (i / 256) / p.blocks}) {
       if (s < 1 || (s > 1 && (s * p.blocks > 640 || s * 4 > steps))) continue;
       const int64_t per = round_up(cdiv(steps, s), 2), parts = cdiv(steps, per), b = parts * p.blocks;
-      const double step = b <= 256 ? 0.27 + 0.24 * P : (double)cdiv(b, 512) * (0.23 + 0.35 * P);
+      const double step = b <= 256 ? 0.25 + 0.22 * P : (double)cdiv(b, 512) * (0.20 + 0.31 * P);
       const double t = (double)per * step + (parts > 1 ? 4.0 + (double)parts * ((double)M * (double)O * (8 / 4.5e6) + 0.06) : 0.0);
       if (s == 1 || t < best) best = t, p.splits = (int)parts, p.steps = (int)per;
     }
