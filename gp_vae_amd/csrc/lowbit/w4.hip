@@ -143,16 +143,17 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
 // Few rows (skinny.hpp) or many (tile.hpp)?  Few: one launch (two where the reduction is split), every group of 64 / P rows
 // decodes all codes, every workgroup stages the operand anew; many: the operand is split into planes first (a launch; none for
 // most bfloat16 operands) and 64 rows share a decoded tile.  Measured on both sides, few / many in us (t: transposed):
-//   bfloat16 16 x 4096 x 32768 25 / 30 (t 37 / 37), 24 x 4096 x 32768 32 / 32 (t 47 / 38), 64 x 4096 x 32768 67 / 39 (t 64 / 41),
-//     64 x 1024 x 4096 12.4 / 11.5, 200 x 512 x 512 8.0 / 9.8, 128 x 512 x 512 t 10.2 / 12.4;
-//   float16 24 x 4096 x 32768 40 / 45 (t 45 / 48), 32 x 8192 x 8192 29 / 29 (t 32 / 32), 64 x 4096 x 32768 55 / 52 (t 92 / 52),
-//     200 x 1024 x 4096 14 / 21 (t 21.7 / 23.5), 96 x 4096 x 32768 94 / 68;
-//   float32 21 x 4096 x 32768 39 / 56 (t 46 / 61), 42 x 1024 x 32768 18 / 27 (t 28 / 36), 42 x 8192 x 8192 54 / 37 (t 60 / 41),
-//     42 x 4096 x 32768 47 / 59 (t 79 / 66), 256 x 1024 x 4096 23 / 26 (t 31 / 29), 128 x 4096 x 4096 34 / 28 (t 39 / 31).
+//   bfloat16 16 x 4096 x 32768 21 / 26 (t 31 / 32), 32 x 4096 x 4096 13.0 / 13.0, 64 x 2048 x 4096 10.9 / 12.3 (t 13.6 / 14.3),
+//     128 x 1024 x 4096 7.6 / 11.6, 200 x 512 x 512 4.7 / 8.4, 24 x 4096 x 32768 32 / 32 (t 47 / 38), 64 x 4096 x 32768 67 / 35;
+//   float16 24 x 4096 x 32768 34 / 40 (t 41 / 45), 32 x 4096 x 8192 20 / 22 (t 21 / 24), 64 x 4096 x 32768 55 / 52 (t 92 / 52),
+//     200 x 1024 x 4096 13.6 / 16.5 (t 20.1 / 21.4), 96 x 4096 x 32768 94 / 68;
+//   float32 21 x 4096 x 32768 35 / 47 (t 44 / 57), 42 x 1024 x 32768 18 / 23 (t 28 / 36), 42 x 4096 x 8192 26 / 25 (t 28 / 29),
+//     42 x 4096 x 32768 49 / 52, 42 x 8192 x 8192 54 / 37 (t 60 / 41), 64 x 4096 x 4096 21.2 / 21.6 (t 22.4 / 25.5),
+//     256 x 1024 x 4096 22.9 / 22.0 (t 28.9 / 27.8), 128 x 4096 x 4096 34 / 28 (t 39 / 31).
 static inline bool use_skinny(int P, int64_t M, int64_t L, int64_t O, bool vjp) {
   const int64_t groups = cdiv(M, SK_MAXROWS / P);
   const double work = (double)P * (double)M * (double)L * (double)O;
-  if (P == 1) return M <= 16 || (groups <= 4 && work <= 0x1p28);
+  if (P == 1) return M <= 16 || (groups <= 4 && work <= 0x1p29);
   if (groups == 1) return P == 3 || M <= 24 || work <= 0x1p32;
   if (groups == 2) return work <= 0x1p32 || (P == 3 && !vjp && O >= 4 * L);
   return groups <= 16 && work <= 3 * 0x1p30;
