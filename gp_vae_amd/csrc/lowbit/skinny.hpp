@@ -8,7 +8,7 @@
 // The image sits in LDS; the waves of a workgroup share it, and split the reduction (WK) as far as there are
 // too few outputs to fill the chip; S workgroups split it further.  Pieces, waves and splits are added in a fixed order.
 // Measured, float32: 1 x 4096 x 32768 13.7 us, 5.0 TB/s (a copy on this card: 4.8); 16 x 4096 x 1024 7.7 us, 37 x 700 x 1025
-// transposed 6.8 us and 1 x 50 x 4096 3.8 us, bound by the chain launch - first loads - products - sums, not by a rate.
+// transposed 6.7 us and 1 x 50 x 4096 3.8 us, bound by the chain launch - first loads - products - sums, not by a rate.
 // More rows: the matrix pipe and the decoding take over (21 x 4096 x 32768 34 us), see use_skinny.
 #pragma once
 #include "frag.hpp"
