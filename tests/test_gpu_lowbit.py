@@ -413,6 +413,19 @@ def test_very_long_reductions(M):
     assert torch.equal(ops.dense_w4(X, w4).double(), want)
 
 
+def test_gradients_of_rows_far_apart():
+    buf = torch.zeros((2, 2 ** 26 + 64), dtype=BF16, device=DEV)
+    buf[:, :5] = torch.arange(1, 11, device=DEV).reshape(2, 5)
+    q = ops.store_q8(torch.ones((2, 3), device=DEV))
+    with pytest.raises(GpvaeError):
+        ops.dense_grads_q8(q, buf[:, :5])                      # more than 2^26 elements from row to row
+    one = ops.store_q8(torch.ones((1, 3), device=DEV))
+    dW, db = ops.dense_grads_q8(one, buf[:1, :5])              # a single row has no distance
+    assert db.tolist() == [1, 2, 3, 4, 5] and dW.tolist() == [[1, 2, 3, 4, 5]] * 3
+    dW, db = ops.dense_grads_q8(q, buf[:, :2 ** 26 - 1][:, -3:].contiguous())
+    assert (dW == 0).all() and (db == 0).all()
+
+
 # ---- streams and graphs -------------------------------------------------------------------------------------------------
 def test_side_stream_and_replayed_graph():
     rng = np.random.default_rng(12)

@@ -127,3 +127,26 @@ def test_oracle_formats():
                 assert np.abs(T - Q).max() <= np.abs(T).max() / 127
         if relu:
             assert ((V > 0) == (X > 0)).all()
+
+
+def test_workspace_queries_of_extreme_sizes():
+    lib = _lib.load_lowbit()
+    sizes = [-5, 0, 1, 2, 31, 33, 128, 129, 1000, 65537, 2 ** 25, 2 ** 30]
+    for name in ("gpvae_dense_w4_workspace_bytes", "gpvae_dense_vjp_w4_workspace_bytes", "gpvae_dense_grads_q8_workspace_bytes"):
+        fn = getattr(lib, name)
+        for dt in (-1, 0, 1, 2, 3, 4):
+            for m in sizes:
+                for k in sizes:
+                    for n in sizes:
+                        w = fn(dt, m, k, n)
+                        assert w >= 0, (name, dt, m, k, n)
+                        if dt in (-1, 1, 4) or min(k, n) < 1 or m < (0 if "grads" in name else 1):
+                            assert w == 0, (name, dt, m, k, n)
+
+
+def test_gradients_refuse_rows_too_far_apart():
+    fn = _lib.load_lowbit().gpvae_dense_grads_q8
+    args = [None, 0, 2, 8, 2 ** 26 + 1, 0, 4096, 4096, 4096, 2 ** 26 + 1, 4096, 2 ** 26 + 1, None, 4096]
+    assert fn(*args) == -5
+    args[4], args[11] = 8, 8
+    assert fn(*args) == -10
