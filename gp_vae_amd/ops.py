@@ -702,6 +702,7 @@ def decoder_vjp_static(dec_params, Z, dF, h0, h1, out=None):
 # handle is fetched without a stream object, pointers are passed as plain integers.
 _LB_DT = {torch.float32: LB_F32, torch.bfloat16: LB_BF16, torch.float16: LB_F16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _lb_dt(what, t):
@@ -715,7 +716,8 @@ def _lb_mat(what, name, t, cols=None, rows=None):
     """A [rows, cols] device matrix the library can read (unit column stride, rows apart), copied if need be."""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         raise GpvaeError("%s: %s must be a 2-D tensor" % (what, name))
-    _dev(t)
+    if not t.is_cuda:
+        _dev(t)
     r, c = t.shape
     if (cols is not None and c != cols) or (rows is not None and r != rows):
         raise GpvaeError("%s: %s must be [%s, %s]; got %s" % (what, name, "rows" if rows is None else rows,
@@ -746,7 +748,7 @@ def _lb_same(what, dev, *ts):
 
 
 def _lb_call(what, dev, fn, *args):
-    if dev == torch.cuda.current_device():
+    if dev == _raw_device():
         rc = fn(_raw_stream(dev), *args)
     else:
         with torch.cuda.device(dev):
@@ -785,7 +787,7 @@ class W4:
                              % (kb, np_, kb, np_ // 8, K, N, tuple(codes.shape), tuple(exps.shape)))
         if codes.dtype != torch.int32 or exps.dtype != torch.uint8 or not (codes.is_contiguous() and exps.is_contiguous()):
             raise GpvaeError("W4: codes must be contiguous int32, exps contiguous uint8")
-        if codes.device != exps.device:
+        if codes.get_device() != exps.get_device():  # (-1: host memory)
             raise GpvaeError("W4: codes on %s, exps on %s" % (codes.device, exps.device))
         self.codes, self.exps, self.K, self.N = codes, exps, K, N
 
@@ -805,7 +807,7 @@ class Q8:
                              % (mb, kp, mb, kp // 8, M, K, tuple(codes.shape), tuple(exps.shape)))
         if codes.dtype != torch.uint8 or exps.dtype != torch.uint8 or not (codes.is_contiguous() and exps.is_contiguous()):
             raise GpvaeError("Q8: codes and exps must be contiguous uint8")
-        if codes.device != exps.device:
+        if codes.get_device() != exps.get_device():  # (-1: host memory)
             raise GpvaeError("Q8: codes on %s, exps on %s" % (codes.device, exps.device))
         self.codes, self.exps, self.M, self.K, self.relu = codes, exps, M, K, bool(relu)
 
