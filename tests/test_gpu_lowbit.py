@@ -462,3 +462,40 @@ def test_side_stream_and_replayed_graph():
             step(Xs[(i + 1) % 4], dYs[(i + 1) % 4])  # the program's own eager work between replays
             torch.cuda.synchronize()
             assert all(torch.equal(a, c) for a, c in zip(outs, want[i])), i
+
+
+# ---- values at the edges of the types ---------------------------------------------------------------------------------
+NAN_BITS = {F32: (torch.int32, [0x7f800001, 0x7f80ffff, 0x7fbfffff, -0x7fffff, -0x7f0001, 0x7fc00000]),
+            BF16: (torch.int16, [0x7f81, 0x7fbf, -0x7f, 0x7fc0]), F16: (torch.int16, [0x7c01, 0x7dff, -0x3ff, 0x7e00])}
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_every_nan_stays_a_nan(M, dt):
+    """Signalling ones too, whose set mantissa bits may all lie below the first bfloat16 piece."""
+    rng = np.random.default_rng(M)
+    K, N = 200, 150
+    w4 = ops.quant_w4(normal(rng, (K, N), F32))
+    X, dY = normal(rng, (M, K), dt), normal(rng, (M, N), dt)
+    bits, patterns = NAN_BITS[dt]
+    A, q = ops.store_q8(X, relu=True)
+    for i, p in enumerate(patterns):
+        for k in (0, 67, K - 1):
+            V = X.clone()
+            V.view(bits)[M - 1, k] = p
+            for src in (V, strided(V)[1]):
+                assert torch.isnan(ops.dense_w4(src, w4, relu=bool(i & 1))[M - 1]).all()
+                assert torch.isfinite(ops.dense_w4(src, w4)[:M - 1]).all()
+            assert torch.isnan(ops.load_q8(ops.store_q8(V))[M - 1, k]) and torch.isnan(ops.load_w4(ops.quant_w4(V))[M - 1, k])
+        for n in (0, 33, N - 1):
+            V = dY.clone()
+            V.view(bits)[M - 1, n] = p
+            for src in (V, strided(V)[1]):
+                dX = ops.dense_vjp_w4(src, w4)
+                assert torch.isnan(dX[M - 1]).all() and torch.isfinite(dX[:M - 1]).all()
+                dX = ops.dense_vjp_w4(src, w4, q)                       # the mask selects: 0 where it is 0
+                assert torch.isnan(dX[M - 1][A[M - 1] > 0]).all() and (dX[A <= 0] == 0).all()
+                dW, db = ops.dense_grads_q8(q, src)
+                rest = [j for j in range(N) if j != n]
+                assert torch.isnan(dW[:, n]).all() and torch.isnan(db[n])
+                assert torch.isfinite(dW[:, rest]).all() and torch.isfinite(db[rest]).all()
