@@ -46,18 +46,16 @@ static inline GradsPlan grads_plan(int P, int64_t M, int64_t K, int64_t N) {
   return p;
 }
 
-// 8 codes (bytes) -> 8 bfloat16 values times 2^e; exponent byte eb (255: NaN)
+// 8 codes (bytes) -> 8 bfloat16 values times 2^e; exponent byte eb (255: NaN).  A signed code is scaled as it is: taken as an
+// offset and a correction of 128 2^e, the correction would overflow at the largest e.
 template <bool RELU> __device__ __forceinline__ u32x4 q8_frag(u32x2 q, uint32_t eb) {
   const float s = scale_of(eb);
   float v[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint32_t w = RELU ? q[h] : q[h] ^ 0x80808080u;  // two's complement -> offset by 128
+    const uint32_t w = q[h];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float u = (float)((w >> (8 * i)) & 255u);
-      v[4 * h + i] = RELU ? u * s : __builtin_fmaf(u, s, -128.0f * s);  // exact: an integer below 256 times 2^e
-    }
+    for (int i = 0; i < 4; ++i) v[4 * h + i] = (RELU ? (float)((w >> (8 * i)) & 255u) : (float)(int8_t)(w >> (8 * i))) * s;  // exact
   }
   return u32x4{pack_hi(v[0], v[1]), pack_hi(v[2], v[3]), pack_hi(v[4], v[5]), pack_hi(v[6], v[7])};
 }

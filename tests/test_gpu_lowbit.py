@@ -499,3 +499,22 @@ def test_every_nan_stays_a_nan(M, dt):
                 rest = [j for j in range(N) if j != n]
                 assert torch.isnan(dW[:, n]).all() and torch.isnan(db[n])
                 assert torch.isfinite(dW[:, rest]).all() and torch.isfinite(db[rest]).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("relu", [False, True])
+def test_gradients_of_the_largest_checkpoints(relu, dt):
+    """Tiles whose power of two is the format's largest, next to zeros: powers of two times them are exact."""
+    M, K, N = 70, 40, 9
+    X = torch.zeros((M, K), device=DEV)
+    X[0, 0], X[1, 1], X[2, 2], X[3, 9], X[20, 17], X[69, 39] = 2e38, -2e38, 3.4e38, 1.7e38, 1.0, -3e38
+    q = ops.store_q8(X, relu=relu)
+    q = q[1] if relu else q
+    assert int(q.exps.max()) == 127 + (120 if relu else 121)
+    dY = torch.zeros((M, N), device=DEV, dtype=dt)
+    for m in (0, 1, 2, 3, 20, 69):
+        dY[m, m % N] = -2.0 ** -(m % 14 + 10)
+    want, S = q8_np(q).T @ np64(dY), np.abs(q8_np(q)).T @ np.abs(np64(dY))
+    dW, db = ops.dense_grads_q8(q, dY)
+    close(dW, want, S, M, F32)
+    close(db, np64(dY).sum(0), np.abs(np64(dY)).sum(0), M, F32)
