@@ -135,6 +135,9 @@ template <typename T, bool VJP> struct Epilogue {
   int64_t act_kp;
   T *out;
   int64_t ldo;
+  Epilogue from_row(int64_t m) const {  // m a multiple of 8
+    return Epilogue{bias, relu, act ? act + m * act_kp : nullptr, act_kp, out + m * ldo, ldo};
+  }
   __device__ __forceinline__ float bias_at(int64_t o) const { return !VJP && bias ? to_f32(bias[o]) : 0.0f; }
   // mask byte of one element; the four bytes of rows m .. m + 3, m a multiple of 4
   __device__ __forceinline__ uint32_t mask_at(int64_t m, int64_t o) const {

@@ -275,7 +275,7 @@ static void launch_grads(hipStream_t st, const GradsPlan &p, int64_t M, int64_t 
   } else {
     launch(grads_kernel<T, RELU, false>);
   }
-  if (split)
+  if (split && hipPeekAtLastError() == hipSuccess)
     hipLaunchKernelGGL(grads_sum_kernel, dim3((unsigned)cdiv(N, 256), (unsigned)(K < 4096 ? K + 1 : 4096)), dim3(256), 0, st, K, N, p.splits, work, dW, lddw, db);
 }
 

@@ -140,7 +140,7 @@ extern "C" int gpvae_store_q8(void *stream, int dtype, int64_t M, int64_t K, con
   LB_REQUIRE(codes && aligned16(codes), 10, "%s: codes must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(exps && aligned16(exps), 11, "%s: exps must be a 16-byte aligned device pointer", fn);
   const int64_t strips = q8_mb(M) * (q8_kp(K) / 4);
-  LB_REQUIRE(cdiv(strips, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+  LB_REQUIRE(launchable(cdiv(strips, 256), 256), 3, "%s: matrix too large", fn);
 #define GO2(T, R)                                                                                                        \
   hipLaunchKernelGGL((store_q8_kernel<T, R>), dim3((unsigned)cdiv(strips, 256)), dim3(256), 0, (hipStream_t)stream, M, K, \
                      (const T *)X, ldx, (T *)Y, ldy, (uint8_t *)codes, (uint8_t *)exps)
@@ -162,7 +162,7 @@ extern "C" int gpvae_load_q8(void *stream, int dtype, int64_t M, int64_t K, int 
   LB_REQUIRE(out, 8, "%s: out is NULL", fn);
   LB_REQUIRE(ldo >= K, 9, "%s: ldo < K", fn);
   const int64_t strips = q8_mb(M) * (q8_kp(K) / 4);
-  LB_REQUIRE(cdiv(strips, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+  LB_REQUIRE(launchable(cdiv(strips, 256), 256), 3, "%s: matrix too large", fn);
   const dim3 grid((unsigned)cdiv(strips, 256));
 #define GO2(T, R)                                                                                                  \
   hipLaunchKernelGGL((load_q8_kernel<T, R>), grid, dim3(256), 0, (hipStream_t)stream, M, K, (const uint8_t *)codes, \
@@ -198,6 +198,7 @@ extern "C" int gpvae_dense_grads_q8(void *stream, int dtype, int64_t M, int64_t 
   LB_REQUIRE(!gpvae_dense_grads_q8_workspace_bytes(dtype, M, K, N) || (work && aligned16(work)), 14,
              "%s: work must be a 16-byte aligned device pointer", fn);
   const GradsPlan p = grads_plan(pieces(dtype), M, K, N);
+  LB_REQUIRE(launchable(p.blocks, GR_THREADS), 4, "%s: K x N too large (%lld tiles of 128 x 128)", fn, (long long)p.blocks);
 #define GO2(T, R)                                                                                                       \
   launch_grads<T, R>((hipStream_t)stream, p, M, K, N, codes, exps, (const T *)dY, lddy, dW, lddw, db, (float *)work)
 #define GO(T) do { if (relu) GO2(T, true); else GO2(T, false); } while (0)

@@ -252,7 +252,7 @@ static void launch_skinny(hipStream_t st, const SkinnyPlan &p, int64_t M, int64_
   else if (p.rt == 3) GO(3);
   else GO(4);
 #undef GO
-  if (p.splits > 1)
+  if (p.splits > 1 && hipPeekAtLastError() == hipSuccess)
     launch_split_sum<T, VJP>(st, M, O, p.splits, part, ep);
 }
 

@@ -264,6 +264,12 @@ struct TilePlan {
   bool direct;         // the operand itself is its only plane
 };
 
+// Rows of one launch; more are taken in turn.  Launches hold fewer than 2^32 threads (a workgroup of split_planes_kernel may have one
+// row, one of tile_kernel 64 rows x 128 of the O outputs), and 2^20 rows fill the chip hundreds of times over.
+static inline int64_t tile_rows(int64_t O) {
+  const int64_t tiles = ((int64_t(1) << 32) / (128 * TL_WM) - 1) / cdiv(O, 128) * (16 * TL_MT * TL_WM);
+  return tiles < 1 ? 16 * TL_MT * TL_WM : tiles < (1 << 20) ? tiles : 1 << 20;
+}
 // Into how many parts is the reduction split?  A step of 64 takes 0.25 + 0.22 P us where a compute unit has one workgroup and
 // 0.20 + 0.31 P us where it has the two that fit, every full round of 512 workgroups anew; a split costs the launch that adds
 // the parts (4 us) and writing and reading them.  The least of that estimate over powers of two and the numbers that give
@@ -302,6 +308,7 @@ static void launch_tile(hipStream_t st, const TilePlan &p, int64_t M, int64_t L,
     while (qsh < 8 && (4 << qsh) < p.Lp) ++qsh;
     hipLaunchKernelGGL((split_planes_kernel<T>), dim3((unsigned)cdiv(M, 256 >> qsh), (unsigned)(p.Lp < 1024 * 65535ll ? cdiv(p.Lp, 1024) : 65535)), dim3(256), 0, st,
                        M, L, p.Lp, qsh, X, ldx, (u32x2 *)work);
+    if (hipPeekAtLastError() != hipSuccess) return;  // reported by the caller; the planes are not written
     planes = reinterpret_cast<const char *>(work);
     rs = 128, ss = M * 128, ps = M * p.Lp * 2;
   }
@@ -309,7 +316,7 @@ static void launch_tile(hipStream_t st, const TilePlan &p, int64_t M, int64_t L,
   const dim3 grid((unsigned)p.blocks, (unsigned)p.splits);
   hipLaunchKernelGGL((tile_kernel<T, VJP>), grid, dim3(128 * TL_WM), 0, st, M, O, planes, rs, ss, ps, (const char *)codes,
                      (const char *)exps, Np, kbs, p.mtiles, p.Lp / 64, p.steps, part, ep);
-  if (p.splits > 1)
+  if (p.splits > 1 && hipPeekAtLastError() == hipSuccess)
     launch_split_sum<T, VJP>(st, M, O, p.splits, part, ep);
 }
 

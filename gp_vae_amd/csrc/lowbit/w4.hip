@@ -110,7 +110,7 @@ extern "C" int gpvae_quant_w4(void *stream, int dtype, int64_t K, int64_t N, con
   LB_REQUIRE(codes && aligned16(codes), 7, "%s: codes must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(exps && aligned16(exps), 8, "%s: exps must be a 16-byte aligned device pointer", fn);
   const int64_t strips = w4_kb(K) * (w4_np(N) / 4);
-  LB_REQUIRE(cdiv(strips, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+  LB_REQUIRE(launchable(cdiv(strips, 256), 256), 3, "%s: matrix too large", fn);
 #define GO(T)                                                                                                         \
   hipLaunchKernelGGL(quant_w4_kernel<T>, dim3((unsigned)cdiv(strips, 256)), dim3(256), 0, (hipStream_t)stream, K, N,  \
                      (const T *)W, ldw, (u32x4 *)codes, (uint32_t *)exps)
@@ -129,7 +129,7 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
   LB_REQUIRE(out, 7, "%s: out is NULL", fn);
   LB_REQUIRE(ldo >= N, 8, "%s: ldo < N", fn);
   const int64_t strips = w4_kb(K) * (w4_np(N) / 4);
-  LB_REQUIRE(cdiv(strips, 256) <= 0x7fffffff, 3, "%s: matrix too large", fn);
+  LB_REQUIRE(launchable(cdiv(strips, 256), 256), 3, "%s: matrix too large", fn);
   const dim3 grid((unsigned)cdiv(strips, 256));
 #define GO(T)                                                                                                     \
   hipLaunchKernelGGL(load_w4_kernel<T>, grid, dim3(256), 0, (hipStream_t)stream, K, N, (const u32x4 *)codes,    \
@@ -165,8 +165,15 @@ static int64_t w4_workspace(int dtype, int64_t M, int64_t L, int64_t O, bool vjp
     const SkinnyPlan p = skinny_plan(P, M, L, O);
     return p.splits > 1 ? p.splits * M * O * 4 : 0;
   }
-  const TilePlan p = tile_plan(P, M, L, O, false);
-  return p.plane_bytes + (p.splits > 1 ? p.splits * M * O * 4 : 0);
+  int64_t most = 0;  // the launches of a call follow one another and share it
+  const int64_t slab = tile_rows(O);
+  for (const int64_t m : {M < slab ? M : slab, M % slab}) {
+    if (m == 0) continue;
+    const TilePlan p = tile_plan(P, m, L, O, false);
+    const int64_t bytes = p.plane_bytes + (p.splits > 1 ? p.splits * m * O * 4 : 0);
+    if (bytes > most) most = bytes;
+  }
+  return most;
 }
 template <typename T, bool VJP>
 static void run_w4(hipStream_t st, int64_t M, int64_t L, int64_t O, const void *X, int64_t ldx, const void *codes,
@@ -178,8 +185,11 @@ static void run_w4(hipStream_t st, int64_t M, int64_t L, int64_t O, const void *
     // a bfloat16 operand is its own plane where its rows can be read 16 bytes at a time to the end of the last step and
     // 256 of them lie within a 32-bit offset
     const bool direct = P == 1 && L % 128 == 0 && ldx % 8 == 0 && ldx < (1 << 23) && aligned16(X);
-    launch_tile<T, VJP>(st, tile_plan(P, M, L, O, direct), M, L, O, (const T *)X, ldx, codes, exps, Np, kbs,
-                        (unsigned char *)work, ep);
+    for (int64_t m = 0, slab = tile_rows(O); m < M; m += slab) {
+      const int64_t rows = M - m < slab ? M - m : slab;
+      launch_tile<T, VJP>(st, tile_plan(P, rows, L, O, direct), rows, L, O, (const T *)X + m * ldx, ldx, codes, exps, Np, kbs,
+                          (unsigned char *)work, ep.from_row(m));
+    }
   }
 }
 extern "C" int64_t gpvae_dense_w4_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {

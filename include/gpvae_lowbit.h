@@ -85,7 +85,7 @@ int gpvae_load_q8(void *stream, int dtype, int64_t M, int64_t K, int relu, const
 /* Parameter gradients of a dense layer y = x W + b from the checkpoint of its input:
  *   dW[k][n] = sum_m X~[m][k] dY[m][n],   db[n] = sum_m dY[m][n]       (float32, overwritten; M = 0: zeros)
  * relu: how the checkpoint was stored.  dY [M, lddy] (dtype); dW [K, lddw]; db [N] may be NULL.  work as above.
- * N and (for M > 1) lddy at most 2^26.                                                                      */
+ * N and (for M > 1) lddy at most 2^26, ceil(K / 128) ceil(N / 128) below 2^23. */
 int64_t gpvae_dense_grads_q8_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N);
 int gpvae_dense_grads_q8(void *stream, int dtype, int64_t M, int64_t K, int64_t N, int relu, const void *codes,
                          const void *exps, const void *dY, int64_t lddy, float *dW, int64_t lddw, float *db, void *work);

@@ -518,3 +518,42 @@ def test_gradients_of_the_largest_checkpoints(relu, dt):
     dW, db = ops.dense_grads_q8(q, dY)
     close(dW, want, S, M, F32)
     close(db, np64(dY).sum(0), np.abs(np64(dY)).sum(0), M, F32)
+
+
+def ends(M, *cuts):
+    """Rows at both ends and on both sides of the cuts."""
+    near = [torch.arange(max(0, c - 9), min(M, c + 9)) for c in (0, *cuts, M)]
+    return torch.cat(near).unique().to(DEV)
+
+
+def test_more_rows_than_a_launch_has_room_for():
+    """2^24 rows of more than 512 reduction indices, a workgroup for each row's pieces: 2^32 threads."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(5)
+    M, K, N = 2 ** 24 + 70, 520, 33
+    X = torch.randn((2 ** 18 + 1, K), device=DEV, generator=g).to(BF16).repeat(65, 1)[:M]
+    w4 = ops.quant_w4(torch.randn((K, N), device=DEV, generator=g))
+    Y, rows, Wd = ops.dense_w4(X, w4), ends(M, 2 ** 20, 2 ** 23, 2 ** 24), ops.load_w4(w4).double()
+    close(Y[rows], (X[rows].double() @ Wd).cpu().numpy(), (X[rows].double().abs() @ Wd.abs()).cpu().numpy(), K, BF16)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_rows_in_several_launches(dt):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(6)
+    M, K, N = 2 ** 20 + 100, 140, 24
+    rand = lambda *s: torch.randn(s, device=DEV, generator=g)
+    w4, wt = ops.quant_w4(rand(K, N)), ops.quant_w4(rand(N, K))  # reductions over 140 both ways
+    X, b, rows = rand(M, K).to(dt), rand(N).to(dt), ends(M, 2 ** 19, 2 ** 20)
+    A, q = ops.store_q8(rand(M, N).to(dt), relu=True)
+    Wd, Wt, Xd = ops.load_w4(w4).double(), ops.load_w4(wt).double().t(), X[rows].double()
+    obuf = torch.full((M + 2, N + 3), 7.0, dtype=dt, device=DEV)
+    out = obuf[1:1 + M, 2:2 + N]
+    ops.dense_w4(X, w4, b, relu=True, out=out)
+    close(out[rows], torch.relu(Xd @ Wd + b.double()).cpu().numpy(), (Xd.abs() @ Wd.abs() + b.double().abs()).cpu().numpy(), K, dt)
+    S = (Xd.abs() @ Wt.abs()).cpu().numpy()
+    ops.dense_vjp_w4(X, wt, q, out=out)
+    close(out[rows], ((Xd @ Wt) * (A[rows] > 0)).cpu().numpy(), S, K, dt)
+    assert (out[A <= 0] == 0).all() and (out[A > 0] != 0).float().mean() > 0.99
+    obuf[1:1 + M, 2:2 + N] = 7.0
+    assert (obuf == 7.0).all()

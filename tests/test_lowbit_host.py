@@ -150,3 +150,17 @@ def test_gradients_refuse_rows_too_far_apart():
     assert fn(*args) == -5
     args[4], args[11] = 8, 8
     assert fn(*args) == -10
+
+
+def test_launches_hold_fewer_than_2_32_threads_in_a_dimension():
+    lib = _lib.load_lowbit()
+    one, big = C.c_void_p(16), 2 ** 20
+    assert lib.gpvae_store_q8(None, 2, big, big, one, big, 0, None, 0, one, one) == -3 and b"too large" in lib.gpvae_lowbit_last_error()
+    assert lib.gpvae_load_q8(None, 2, big, big, 0, one, one, one, big) == -3
+    assert lib.gpvae_quant_w4(None, 2, 2 ** 23, 2 ** 20, one, 2 ** 20, one, one) == -3
+    assert lib.gpvae_load_w4(None, 2, 2 ** 23, 2 ** 20, one, one, one, 2 ** 20) == -3
+    assert lib.gpvae_dense_grads_q8(None, 0, 1, 2 ** 30, 1, 0, one, one, one, 1, one, 1, None, one) == -4
+    # many rows are taken in several launches, which share one workspace
+    for fn, k, n in ((lib.gpvae_dense_w4_workspace_bytes, 640, 50), (lib.gpvae_dense_vjp_w4_workspace_bytes, 50, 640)):
+        for rows in (2 ** 24, 2 ** 24 + 70, 2 ** 30):
+            assert fn(0, rows, k, n) == fn(0, 2 ** 20, k, n) == 3 * 2 ** 20 * 640 * 2
