@@ -557,3 +557,80 @@ def test_rows_in_several_launches(dt):
     assert (out[A <= 0] == 0).all() and (out[A > 0] != 0).float().mean() > 0.99
     obuf[1:1 + M, 2:2 + N] = 7.0
     assert (obuf == 7.0).all()
+
+
+# Reductions split over workgroups, whose parts a second launch adds and finishes, by few and by many rows
+SPLIT = [(1, 32768, 130), (1, 9000, 33), (3, 8192, 200), (21, 5000, 97), (40, 9001, 65), (130, 9000, 260), (300, 6000, 130),
+         (700, 4100, 300), (1024, 4096, 1024)]
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,L,O", SPLIT)
+def test_split_reductions_in_both_directions(M, L, O, dt):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(M + L + O)
+    rand = lambda *s: torch.randn(s, device=DEV, generator=g)
+    w4, wt = ops.quant_w4(rand(L, O) * L ** -0.5), ops.quant_w4(rand(O, L) * L ** -0.5)
+    X, b = rand(M, L).to(dt), rand(O).to(dt)
+    A, q = ops.store_q8(rand(M, O).to(dt), relu=True)
+    lib, code = ops._lib.load_lowbit(), ops._LB_DT[dt]
+    work = lib.gpvae_dense_w4_workspace_bytes(code, M, L, O), lib.gpvae_dense_vjp_w4_workspace_bytes(code, M, O, L)
+    assert min(work) >= 2 * M * O * 4
+    obuf = torch.full((M + 1, O + 3), 7.0, dtype=dt, device=DEV)
+    out = obuf[:M, 2:2 + O]
+    Wd, Wt, Xd, bd = ops.load_w4(w4).double(), ops.load_w4(wt).double().t(), X.double(), b.double()
+    for bias, relu in ((None, False), (b, False), (b, True)):
+        want, S = Xd @ Wd + (0 if bias is None else bd), Xd.abs() @ Wd.abs() + (0 if bias is None else bd.abs())
+        torch.full((max(work) // 4,), float("nan"), device=DEV)  # whatever the workspace held before
+        ops.dense_w4(X, w4, bias, relu=relu, out=out)
+        close(out, (torch.relu(want) if relu else want).cpu().numpy(), S.cpu().numpy(), L, dt)
+        assert torch.equal(out, ops.dense_w4(strided(X)[1], w4, bias, relu=relu))
+    want, S = Xd @ Wt, Xd.abs() @ Wt.abs()
+    for act in (None, q):
+        torch.full((max(work) // 4,), float("nan"), device=DEV)
+        ops.dense_vjp_w4(X, wt, act, out=out)
+        close(out, (want if act is None else want * (A > 0)).cpu().numpy(), S.cpu().numpy(), L, dt)
+        assert torch.equal(out, ops.dense_vjp_w4(strided(X)[1], wt, act))
+    assert (out[A <= 0] == 0).all()
+    X[M - 1, L - 1] = float("inf")  # the mask selects: what it hides is 0 whatever it is
+    ops.dense_vjp_w4(X, wt, q, out=out)
+    hit = (A[M - 1] > 0) & (ops.load_w4(wt)[:, L - 1] != 0)
+    assert (out[A <= 0] == 0).all() and torch.isinf(out[M - 1][hit]).all() and torch.isfinite(out[:M - 1]).all()
+    obuf[:M, 2:2 + O] = 7.0
+    assert (obuf == 7.0).all()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("M,K,N", [(2000, 300, 200), (1111, 130, 257), (4096, 40, 1000)])
+def test_gradients_whose_rows_are_split(M, K, N, dt):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(M + K + N)
+    dY = torch.randn((M, N), device=DEV, generator=g).to(dt)
+    work = ops._lib.load_lowbit().gpvae_dense_grads_q8_workspace_bytes(ops._LB_DT[dt], M, K, N)
+    assert work >= 2 * (K + 1) * N * 4
+    for relu in (False, True):
+        q = ops.store_q8(torch.randn((M, K), device=DEV, generator=g), relu=relu)
+        q = q[1] if relu else q
+        V, D = ops.load_q8(q).double(), dY.double()
+        obuf = torch.full((K + 1, N + 3), 7.0, device=DEV)
+        out = obuf[:K, 2:2 + N], torch.empty(N, device=DEV)
+        torch.full((work // 4,), float("nan"), device=DEV)
+        dW, db = ops.dense_grads_q8(q, dY, out=out)
+        close(dW, (V.t() @ D).cpu().numpy(), (V.abs().t() @ D.abs()).cpu().numpy(), M, F32)
+        close(db, D.sum(0).cpu().numpy(), D.abs().sum(0).cpu().numpy(), M, F32)
+        assert torch.equal(dW, ops.dense_grads_q8(q, strided(dY)[1])[0])
+        obuf[:K, 2:2 + N] = 7.0
+        assert (obuf == 7.0).all()
+
+
+def test_bfloat16_operands_past_32_bits_read_in_place():
+    """Rows of whole steps of 128: the tiles read the operand itself, more than 2^32 bytes of it."""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(7)
+    M, L, O = 33000, 65664, 40
+    X = torch.randn((M, L), device=DEV, generator=g, dtype=BF16)
+    assert X.numel() * 2 > 2 ** 32
+    w4, wt, rows = ops.quant_w4(torch.randn((L, O), device=DEV, generator=g)), ops.quant_w4(torch.randn((O, L), device=DEV, generator=g)), ends(M, 2 ** 15)
+    Xd = X[rows].double()
+    for got, W in ((ops.dense_w4(X, w4), ops.load_w4(w4).double()), (ops.dense_vjp_w4(X, wt), ops.load_w4(wt).double().t())):
+        close(got[rows], (Xd @ W).cpu().numpy(), (Xd.abs() @ W.abs()).cpu().numpy(), L, BF16)
