@@ -7,9 +7,10 @@
 // row p M + m of the operand image is piece p of row m, so one row of float32 costs one matrix instruction, not three.
 // The image sits in LDS; the waves of a workgroup share it, and split the reduction (WK) as far as there are
 // too few outputs to fill the chip; S workgroups split it further.  Pieces, waves and splits are added in a fixed order.
-// Measured, float32: 1 x 4096 x 32768 13.7 us, 5.0 TB/s (a copy on this card: 4.8); 16 x 4096 x 1024 7.7 us, 37 x 700 x 1025
-// transposed 6.7 us and 1 x 50 x 4096 3.8 us, bound by the chain launch - first loads - products - sums, not by a rate.
-// More rows: the matrix pipe and the decoding take over (21 x 4096 x 32768 34 us), see use_skinny.
+// Measured, float32: 1 x 4096 x 32768 17.0-19.4 us with the codes in memory (4.1-3.6 TB/s; a copy on this card: 4.8), 14.0 with
+// part of them in the last-level cache; 16 x 4096 x 1024 7.7 us, 37 x 700 x 1025 transposed 6.7 us and 1 x 50 x 4096 4.2 us, bound by the
+// chain launch - first loads - products - sums, not by a rate.  More rows: staging, the matrix pipe and the decoding take over
+// (21 x 4096 x 32768 35 us; the image is written, waited for and multiplied in turn), see use_skinny.
 #pragma once
 #include "frag.hpp"
 
@@ -32,11 +33,11 @@ static constexpr int skinny_lds(int rt) { return rt <= 1 ? 40 << 10 : rt == 2 ? 
 static inline SkinnyPlan skinny_plan(int P, int64_t M, int64_t L, int64_t O) {
   SkinnyPlan p;
   const int64_t steps = cdiv(L, 128), tiles = cdiv(O, 32);
-  // Smaller groups than fit where that leaves the chip idle: each decodes all codes again, but stages fewer rows.  Up to 256
-  // workgroups for a short reduction, 128 for a longer one; beyond, splitting the reduction is better.  Before / after: float32
-  // 37 x 700 x 1025 transposed 12.1 / 6.8 us, bfloat16 60 rows 13.3 / 7.7, 64 x 4000 x 200 14.1 / 10.9; where it is not
-  // done: float32 128 x 1024 x 4096 transposed 18.8 (22.2 with twice as many), 42 x 8192 x 2048 17.9 (21.8).
-  const int64_t most_blocks = steps <= 9 ? 128 : steps <= 32 ? 64 : 0;
+  // Smaller groups than fit where that leaves the chip idle: each decodes all codes again, but stages fewer rows.  Doubled while
+  // there are at most 128 workgroups for a reduction of up to 16 steps, 64 for one of up to 32; beyond, splitting the reduction
+  // is better.  Limits of 0 / 64 / 128, float32 40 rows x 1000 outputs: 9 steps 12.0 / 6.3 / 6.3 us, 32 steps 10.4 / 8.2 / 8.2 (float16 62 rows x 700:
+  // 40 steps 15.1 / 15.9 / 15.9); 3000 outputs: 7 steps 10.4 (64) / 7.9 (128), 14 steps 13.6 / 11.9, 20 steps 14.4 / 15.5, 30 steps 17.5 / 19.2.
+  const int64_t most_blocks = steps <= 16 ? 128 : steps <= 32 ? 64 : 0;
   int rows, room;
   for (p.groups = (int)cdiv(M, SK_MAXROWS / P);; p.groups *= 2) {
     p.mg = (int)cdiv(M, p.groups);
@@ -50,8 +51,10 @@ static inline SkinnyPlan skinny_plan(int P, int64_t M, int64_t L, int64_t O) {
     if (p.rt == 1 || p.gx * p.groups > most_blocks) break;
   }
   int64_t s = p.gx * p.groups < 256 ? cdiv(512, p.gx * p.groups) : 1;
-  // a split costs a second launch (3 us): worth it down to four steps of each wave for one operand tile, to one for three or
-  // four, whose steps take longer (16 x 1024 x 4096 transposed: 15.0 us at four, 11.2 at two, 9.5 at one; 1 x 4096 x 1024: 5.5, 6.7, 6.3)
+  // a split costs a second launch (3 us): worth it down to four steps of each wave for one operand tile, two for two, one for
+  // three or four, whose steps take longer.  At four / two / one: float32 1 x 4096 x 1024 5.6 / 6.7 / 6.3 us, 16 x 1024 x 4096 transposed
+  // 9.3 / 8.9 / 9.3, float16 40 x 8192 x 500 13.7 / 10.5 / 9.8.  Longer reductions of one or two operand tiles would bear a finer split:
+  // bfloat16 8 x 8192 x 512 9.0 / 7.3 / 6.6, 24 x 500 x 8192 transposed 14.4 / 10.3 / 8.3.
   const int64_t most = steps / ((p.rt == 1 ? 4 : p.rt == 2 ? 2 : 1) * p.wk);
   if (s > most) s = most;
   if (s < 1) s = 1;

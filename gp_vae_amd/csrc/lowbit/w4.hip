@@ -143,19 +143,23 @@ extern "C" int gpvae_load_w4(void *stream, int dtype, int64_t K, int64_t N, cons
 // Few rows (skinny.hpp) or many (tile.hpp)?  Few: one launch (two where the reduction is split), every group of 64 / P rows
 // decodes all codes, every workgroup stages the operand anew; many: the operand is split into planes first (a launch; none for
 // most bfloat16 operands) and 64 rows share a decoded tile.  Measured on both sides, few / many in us (t: transposed):
-//   bfloat16 16 x 4096 x 32768 21 / 26 (t 31 / 32), 32 x 4096 x 4096 13.0 / 13.0, 64 x 2048 x 4096 10.9 / 12.3 (t 13.6 / 14.3),
-//     128 x 1024 x 4096 7.6 / 11.6, 200 x 512 x 512 4.7 / 8.4, 24 x 4096 x 32768 32 / 32 (t 47 / 38), 64 x 4096 x 32768 67 / 35;
-//   float16 24 x 4096 x 32768 34 / 40 (t 41 / 45), 32 x 4096 x 8192 20 / 22 (t 21 / 24), 64 x 4096 x 32768 55 / 52 (t 92 / 52),
-//     200 x 1024 x 4096 13.6 / 16.5 (t 20.1 / 21.4), 96 x 4096 x 32768 94 / 68;
-//   float32 21 x 4096 x 32768 35 / 47 (t 44 / 57), 42 x 1024 x 32768 18 / 23 (t 28 / 36), 42 x 4096 x 8192 26 / 25 (t 28 / 29),
-//     42 x 4096 x 32768 49 / 52, 42 x 8192 x 8192 54 / 37 (t 60 / 41), 64 x 4096 x 4096 21.2 / 21.6 (t 22.4 / 25.5),
-//     256 x 1024 x 4096 22.9 / 22.0 (t 28.9 / 27.8), 128 x 4096 x 4096 34 / 28 (t 39 / 31).
+//   bfloat16 16 x 4096 x 32768 21.2 / 26.2 (t 31.1 / 32.2), 32 x 4096 x 4096 13.0 / 13.0, 64 x 2048 x 4096 10.9 / 12.4 (t 11.3 / 14.4),
+//     128 x 1024 x 4096 7.7 / 11.7 (t 13.9 / 14.3), 200 x 512 x 512 4.8 / 8.5, 24 x 4096 x 32768 25.9 / 28.4 (t 38.8 / 33.6),
+//     64 x 4096 x 32768 49 / 35.6 (t 52 / 38.7);
+//   float16 24 x 4096 x 32768 34 / 40 (t 40 / 44), 32 x 4096 x 8192 20.0 / 22.0 (t 21.1 / 23.7), 64 x 4096 x 32768 50 / 47 (t 81 / 51),
+//     200 x 1024 x 4096 13.5 / 16.5 (t 19.8 / 21.5), 96 x 4096 x 32768 79 / 63 (t 148 / 80);
+//   float32 21 x 4096 x 32768 35 / 47 (t 45 / 55), 42 x 1024 x 32768 18.4 / 22.0 (t 29 / 36), 42 x 4096 x 8192 25.9 / 24.4 (t 27.8 / 28.1),
+//     42 x 4096 x 32768 49 / 51 (t 76 / 60), 42 x 8192 x 65536 152 / 160, 42 x 8192 x 32768 95 / 91, 42 x 8192 x 8192 44 / 32.5
+//     (t 50 / 39), 64 x 4096 x 4096 21.6 / 21.8 (t 24.0 / 25.7), 256 x 1024 x 4096 23.2 / 22.0 (t 29.3 / 27.8),
+//     128 x 4096 x 4096 32.7 / 25.8 (t 37.8 / 30.5).
+// The rule takes the slower side of these for bfloat16 24 x 4096 x 32768 (by 10 %, so that its transposed product is not
+// 15 % slower), float32 42 x 4096 x 8192 and 256 x 1024 x 4096 (by 6 %).
 static inline bool use_skinny(int P, int64_t M, int64_t L, int64_t O, bool vjp) {
   const int64_t groups = cdiv(M, SK_MAXROWS / P);
   const double work = (double)P * (double)M * (double)L * (double)O;
   if (P == 1) return M <= 16 || (groups <= 4 && work <= 0x1p29);
   if (groups == 1) return P == 3 || M <= 24 || work <= 0x1p32;
-  if (groups == 2) return work <= 0x1p32 || (P == 3 && !vjp && O >= 4 * L);
+  if (groups == 2) return work <= 0x1p32 || (P == 3 && !vjp && O >= 8 * L);
   return groups <= 16 && work <= 3 * 0x1p30;
 }
 static int64_t w4_workspace(int dtype, int64_t M, int64_t L, int64_t O, bool vjp) {
