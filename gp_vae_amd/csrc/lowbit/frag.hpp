@@ -69,7 +69,7 @@ struct Tr8 {
 // the value clamped to the finite range, so that inf * w stays inf (inf - inf would make it NaN).  A float32 NaN is made a
 // quiet one first: a signalling one may have its mantissa bits in the lower half only, and its upper half is an infinity.
 // That instruction a value costs dense_grads_q8 4096 x 1024 x 4096 103.8 -> 107.4 us, dense_vjp_w4 42 x 1024 x 32768 27.8 -> 28.6 us,
-// and nothing measurable where the rows are split once or few.  (float16: the conversion to float32 quiets.)
+// and nothing measurable where rows are split once or are few.  (float16: the conversion to float32 quiets.)
 template <typename T> struct Split;
 __device__ __forceinline__ uint32_t pack_hi(float a, float b) {  // top halves of a (low) and b (high)
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);

@@ -6,8 +6,8 @@
 // LDS: a thread loads 8 consecutive rows of a column (consecutive lanes: consecutive columns), splits them into their
 // bfloat16 pieces and writes each piece's 8 values as 16 bytes.  One 128 x 128 tile per workgroup, 64 rows a step, loaded
 // one step ahead through buffer descriptors: scalar bases, and rows past the end read as zero without a test.
-// float32 is bound by matrix and vector instructions, of which little overlaps (4096 x 1024 x 4096: 43 % and 37 % of the time; 103 us,
-// 1000 TFLOP/s over the three pieces), the other types by instruction issue, LDS and the step's barrier (bfloat16 50 us, float16
+// float32 is bound by matrix and vector instructions, of which little overlaps (4096 x 1024 x 4096: 43 % and 37 % of the time; 103-107 us,
+// 960-1000 TFLOP/s over the three pieces), the other types by instruction issue, LDS and the step's barrier (bfloat16 50 us, float16
 // 74 us; a library product of two bfloat16 matrices of this size: 52 us).  All row tiles of a column tile run on one
 // XCD (xcd_chunk), whose L2 then serves dY to them: dealt round-robin every XCD read all of dY from memory (140 us before,
 // 122 after).  Tried without gain: 4 steps in flight, the two waves of a SIMD half a step apart, matrix and vector instructions
@@ -26,7 +26,7 @@ struct GradsPlan {
 // Into how many parts are the rows split?  A step takes 0.35 + 0.38 P us (P pieces of dY), every full round of 256 workgroups
 // anew; a split costs the launch that adds the parts (4 us) and writing and reading them.  The least of that estimate over
 // powers of two and the number that gives every unit a workgroup.  Measured, one part / two / four: bfloat16 300 x 700 x 1001
-// 10.1 / 15.4 / 15.1 us, float32 300 x 700 x 1000 13.7 / 18.0 / 16.7, 2000 x 1024 x 1024 50 / 37.5 / 28.
+// 10.1 / 15.2 / 15.0 us, float32 300 x 700 x 1000 14.2 / 18.3 / 17.0, 2000 x 1024 x 1024 52 / 39 / 28.5.
 static inline GradsPlan grads_plan(int P, int64_t M, int64_t K, int64_t N) {
   GradsPlan p;
   p.ktiles = (int)cdiv(K, 128);

@@ -7,7 +7,7 @@ namespace gpvae_lb {
 // tile: 8 loads of 4 elements (16 bytes of float32) cover the strip, the tile's largest magnitude is one exchange with the
 // neighbouring lane, and its 4 columns of codes are 32 consecutive bytes.  Consecutive lanes take consecutive
 // strips of the same rows, so that every row of a wave is one contiguous stretch.  Measured, float32 4096 x 4096 with the
-// ReLU's output: 26.3 us, 5.7 TB/s (the matrices fit the last-level cache; 16384 x 4096 with the reader: 187 us, 5.0 TB/s).
+// ReLU's output: 26.2 us, 5.8 TB/s (the matrices fit the last-level cache; 16384 x 4096 with the reader: 188 us, 5.0 TB/s).
 template <typename T, bool RELU>
 __global__ __launch_bounds__(256) void store_q8_kernel(int64_t M, int64_t K, const T *X, int64_t ldx, T *Y, int64_t ldy,
                                                        uint8_t *__restrict__ codes, uint8_t *__restrict__ exps) {
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void store_q8_kernel(int64_t M, int64_t K, con
   if ((id & 1) == 0) exps[mb * (Kp / 8) + k0 / 8] = (uint8_t)eb;
 }
 
-// The reverse: a thread reads its strip's 32 bytes of codes and writes 8 rows of 4 elements (4096 x 4096: 15.7 us, 5.3 TB/s).
+// The reverse: a thread reads its strip's 32 bytes of codes and writes 8 rows of 4 elements (4096 x 4096: 15.5 us, 5.4 TB/s).
 template <typename T, bool RELU>
 __global__ __launch_bounds__(256) void load_q8_kernel(int64_t M, int64_t K, const uint8_t *__restrict__ codes,
                                                       const uint8_t *__restrict__ exps, T *__restrict__ out, int64_t ldo) {

@@ -5,10 +5,11 @@
 // vector instructions compete with the matrix ones) and staged through LDS, double buffered, 64 reduction indices at a time,
 // 16-byte chunks at chunk ^ (row / 2 % 8) so that fragment reads and stage writes are free of bank conflicts; the codes go
 // straight from memory to registers, one step ahead, and are decoded a half step before they are used.
-// Measured, float32 (three pieces): 1024 x 4096 x 4096 91 us in all, the tiles alone 83, 1240 TFLOP/s issued (a library product of
-// two 8192 x 8192 bfloat16 matrices: 1213).  1024 x 1024 x 4096 34 us: tiles 28.9, of which 11 do not depend on the depth
-// (launch, first loads, last stores), planes 5.5; transposed 48 us with 8.1 for the planes and 6.8 for the sum of four parts.
-// bfloat16 (in place) 4096 x 4096 x 4096 143 us, 963 TFLOP/s.  Before the halves of a step were interleaved (all reads, all
+// Measured, float32 (three pieces): 1024 x 4096 x 4096 87-91 us in all, the tiles alone 83, 1240 TFLOP/s issued (a library product
+// of two 8192 x 8192 bfloat16 matrices: 1213).  1024 x 1024 x 4096 33 us: tiles 28.1, of which 11 do not depend on the depth
+// (launch, first loads, last stores), planes 5.5; transposed 45 us: tiles 31.4, planes 8.0 and the sum of four parts 6.6.
+// 4096 x 4096 x 4096 bfloat16 (in place) 140 us, 983 TFLOP/s, transposed 179; float16 235 us, 1170 TFLOP/s over its two pieces.  1024 x 1024 x 4096
+// transposed: bfloat16 27 us, float16 35, most of it the parts and their sum.  Before the halves of a step were interleaved (all reads, all
 // decoding, all products, all writes) and addresses took 50 instructions a step: 104, 36.7 and 50.2 us.  Tiles of 128 rows
 // (wave tiles 64 x 64, one workgroup a unit): 125 and 41.
 #pragma once
@@ -273,8 +274,9 @@ static inline int64_t tile_rows(int64_t O) {
 // Into how many parts is the reduction split?  A step of 64 takes 0.25 + 0.22 P us where a compute unit has one workgroup and
 // 0.20 + 0.31 P us where it has the two that fit, every full round of 512 workgroups anew; a split costs the launch that adds
 // the parts (4 us) and writing and reading them.  The least of that estimate over powers of two and the numbers that give
-// every unit one or two workgroups.  Measured, one part / two / four: float32 512 x 1024 x 4096 23 / 32 / 35 us,
-// 512 x 4096 x 4096 60.5 / 60.5 / 65, 1024 x 1024 x 4096 transposed 69 / 50 / 48; bfloat16 1024 x 1000 x 1000 14.6 / 20.5 / 23.6.
+// every unit one or two workgroups.  Measured, one part / two / four: float32 512 x 1024 x 4096 24.6 / 32.7 / 36.4 us,
+// 512 x 4096 x 4096 58 / 59 / 63, 1024 x 1024 x 4096 transposed 68.6 / 51.3 / 47.8 (bfloat16 40.4 / 31.9 / 28.4); bfloat16 1024 x 1000 x 1000
+// 14.6 / 20.6 / 23.5.
 static inline TilePlan tile_plan(int P, int64_t M, int64_t L, int64_t O, bool direct) {
   TilePlan p;
   p.direct = direct;

@@ -6,7 +6,7 @@ namespace gpvae_lb {
 
 // Bound by memory: W is read once.  A thread owns 32 rows x 4 columns, half of four tiles: rows are read 4 elements at a time
 // (consecutive lanes: consecutive columns), a tile's largest magnitude is one exchange with the neighbouring lane, and
-// the codes of its 4 columns are 64 consecutive bytes.  Measured, float32 4096 x 32768: 168 us, 3.6 TB/s.
+// the codes of its 4 columns are 64 consecutive bytes.  Measured, float32 4096 x 32768: 160 us, 3.8 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void quant_w4_kernel(int64_t K, int64_t N, const T *__restrict__ W, int64_t ldw,
                                                        u32x4 *__restrict__ codes, uint32_t *__restrict__ exps) {
@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void quant_w4_kernel(int64_t K, int64_t N, con
   if ((id & 1) == 0) exps[kb * (Np / 8) + n0 / 8] = eall;
 }
 
-// The reverse: a thread reads the 64 bytes of its 4 columns and writes 32 rows of 4 elements (4096 x 32768: 143 us, 4.2 TB/s).
+// The reverse: a thread reads the 64 bytes of its 4 columns and writes 32 rows of 4 elements (4096 x 32768: 141 us, 4.3 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void load_w4_kernel(int64_t K, int64_t N, const u32x4 *__restrict__ codes,
                                                       const uint32_t *__restrict__ exps, T *__restrict__ out, int64_t ldo) {

@@ -857,7 +857,8 @@ def dense_w4(X, w4, bias=None, relu=False, out=None):
 
 def dense_vjp_w4(dY, w4, act=None, out=None):
     """dX = dY W^T [M, K] for dY [M, N] and weights in 4 bits.  act: the :class:`Q8` checkpoint (relu=True) of the layer's
-    input; dX is then also multiplied by its mask (input > 0), i.e. it is the gradient before the ReLU that made the input.
+    input; dX is then 0 where the input is not positive, whatever the product is there, i.e. it is the gradient before the
+    ReLU that made the input.
     out, if given, must not overlap dY."""
     K, N = w4.K, w4.N
     dY = _lb_mat("dense_vjp_w4", "dY", dY, cols=N)
@@ -879,7 +880,8 @@ def dense_vjp_w4(dY, w4, act=None, out=None):
 
 def store_q8(X, relu=False, out=None):
     """8-bit checkpoint of X [M, K] (float32, bfloat16 or float16), one power of two per 8 x 8 tile: a :class:`Q8`.
-    relu=True: (Y, Q8) with Y = max(X, 0), written to `out` if given (X itself: in place), and the checkpoint of Y.
+    relu=True: (Y, Q8) with Y = max(X, 0), written to `out` if given (X itself: in place; it must not
+    overlap X otherwise), and the checkpoint of Y.
     A tile with an infinity or a NaN reads as NaN; its ReLU mask stays that of the values (NaN passes)."""
     src = X
     X = _lb_mat("store_q8", "X", X)
@@ -919,7 +921,7 @@ def load_q8(q8, dtype=torch.float32):
 def dense_grads_q8(q8, dY, out=None):
     """(dW [K, N], db [N]) float32 of a dense layer y = x W + b from the 8-bit checkpoint of its input x [M, K] and
     dY [M, N] (float32, bfloat16 or float16): dW = x~^T dY, db = sum of dY's rows.  out: optional pair (dW, db) of float32
-    tensors to write to, not overlapping dY (db may be None: not wanted)."""
+    tensors to write to, not overlapping dY or each other (db may be None: not wanted)."""
     M, K = q8.M, q8.K
     dY = _lb_mat("dense_grads_q8", "dY", dY, rows=M)
     dt, dev, N = _lb_dt("dense_grads_q8", dY), dY.get_device(), dY.shape[1]

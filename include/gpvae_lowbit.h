@@ -61,9 +61,10 @@ int64_t gpvae_dense_w4_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t 
 int gpvae_dense_w4(void *stream, int dtype, int64_t M, int64_t K, int64_t N, const void *X, int64_t ldx,
                    const void *codes, const void *exps, const void *bias, int relu, void *Y, int64_t ldy, void *work);
 
-/* The product with the transposed weights: dX[m][k] = (sum_n dY[m][n] W~[k][n]) * mask[m][k].
- * act_codes: the q8 codes of the layer's input A [M, K] stored with relu != 0; mask = (code != 0), i.e. A > 0, so dX
- * is the gradient BEFORE the previous layer's ReLU.  act_codes NULL: no mask.                               */
+/* The product with the transposed weights: dX[m][k] = sum_n dY[m][n] W~[k][n] where mask[m][k], 0 elsewhere (whatever
+ * the sum is there, an infinity or a NaN too).  dY [M, lddy], dX [M, lddx], not overlapping.
+ * act_codes: the q8 codes of the layer's input A [M, K] stored with relu != 0; mask = (code != 0), i.e. A > 0 or NaN, so
+ * dX is the gradient BEFORE the previous layer's ReLU.  act_codes NULL: no mask.                            */
 int64_t gpvae_dense_vjp_w4_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N);
 int gpvae_dense_vjp_w4(void *stream, int dtype, int64_t M, int64_t K, int64_t N, const void *dY, int64_t lddy,
                        const void *codes, const void *exps, const void *act_codes, void *dX, int64_t lddx, void *work);
@@ -72,7 +73,7 @@ int gpvae_dense_vjp_w4(void *stream, int dtype, int64_t M, int64_t K, int64_t N,
  * gpvae_store_q8   relu == 0: the checkpoint of X [M, ldx] (nearest, ties to even; Y must be NULL).
  *                  relu != 0: Y = max(X, 0) (NaN stays NaN) and the checkpoint of Y, codes 0 .. 255; a positive
  *                  value never becomes code 0, so (code != 0) is the ReLU's mask.  Y [M, ldy] may be NULL, or X
- *                  itself (ldy == ldx).
+ *                  itself (ldy == ldx), and must not overlap X otherwise.
  * gpvae_load_q8    the values X~ the checkpoint stands for, out [M, ldo] (exact in float32; exact in bfloat16).
  * M = 0 is an empty checkpoint; K >= 1.                                                                     */
 int64_t gpvae_q8_code_bytes(int64_t M, int64_t K);
@@ -84,6 +85,7 @@ int gpvae_load_q8(void *stream, int dtype, int64_t M, int64_t K, int relu, const
 
 /* Parameter gradients of a dense layer y = x W + b from the checkpoint of its input:
  *   dW[k][n] = sum_m X~[m][k] dY[m][n],   db[n] = sum_m dY[m][n]       (float32, overwritten; M = 0: zeros)
+ * dW and db must not overlap dY or each other.
  * relu: how the checkpoint was stored.  dY [M, lddy] (dtype); dW [K, lddw]; db [N] may be NULL.  work as above.
  * N and (for M > 1) lddy at most 2^26, ceil(K / 128) ceil(N / 128) below 2^23. */
 int64_t gpvae_dense_grads_q8_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N);
