@@ -224,3 +224,36 @@ def test_refusals():
     with pytest.raises(ValueError):
         VAEInference(None, lst, z, 1, np.arange(n) / n, np.zeros(n), [1, 2], {}, weights="w8")
     assert math.isfinite(float(F.sum()))
+
+
+def test_inference_with_a_decoder_wider_than_the_float_one():
+    """Hidden widths above 1024: predictions, and the potential's gradient against autograd in 64 bits."""
+    rng = np.random.default_rng(21)
+    n, h0, h1, z = 500, 1200, 1100, 12
+    p = params(rng, n, h0, h1, z)
+    x, obs = np.arange(n) / n, [3, 77, 78, 250, 499]
+    y = np.cos(5 * x)
+    inf = VAEInference(None, [(p["V1"], p["c1"]), (), (p["V2"], p["c2"]), (), (p["V3"], p["c3"])], z, 1, x, y, obs, {}, weights="w4")
+    W = [ops.load_w4(w).double() for w in inf.dec_w4.layers]
+    b = [t.double() for t in inf.dec_w4.biases]
+    Z = torch.tensor(rng.standard_normal((7, z)), dtype=torch.float32, device=DEV)
+    u = torch.tensor(np.log(rng.uniform(0.1, 0.3, 7)), dtype=torch.float32, device=DEV)
+    y1, e1 = layer(np64(Z), 0 * np64(Z), np64(W[0]), np64(b[0]))
+    y2, e2 = layer(np.maximum(y1, 0), e1, np64(W[1]), np64(b[1]))
+    f, ef = layer(np.maximum(y2, 0), e2, np64(W[2]), np64(b[2]))
+    within(inf.predict(Z), f, ef)
+    zd, ud = Z.double().requires_grad_(), u.double().requires_grad_()
+    F = torch.relu(torch.relu(zd @ W[0] + b[0]) @ W[1] + b[1]) @ W[2] + b[2]
+    r = F[:, obs] - inf.y.double()[obs]
+    s = torch.exp(ud)
+    U = 0.5 * (r * r).sum(1) / s ** 2 + len(obs) * ud + 0.5 * (zd * zd).sum(1) + 0.5 * (s / 0.1) ** 2 - ud
+    U.sum().backward()
+    got = inf.potential_and_grad(Z, u)
+    # the residual's error e counts (|r| + e) e / s^2 in U; float32 sums of fewer than 32 terms and exp add 64 eps of the terms
+    s2, rr = np.exp(2 * np64(u))[:, None], np.abs(np64(r))
+    const = (got[0].double() - U).detach()  # the potential's constant terms
+    tol = ((rr + ef[:, obs]) * ef[:, obs] / s2).sum(1) + 64 * 2 * U.detach().abs().cpu().numpy() * 2.0 ** -23 + 64 * 2.0 ** -23 * ((rr ** 2 / s2).sum(1) + 100)
+    assert (np.abs(np64(const - const.mean())) <= tol + tol.mean()).all()
+    # gradients: relative to the largest, as above
+    assert np.abs(np64(got[1]) - np64(zd.grad)).max() <= 1e-4 * np.abs(np64(zd.grad)).max()
+    assert np.abs(np64(got[2]) - np64(ud.grad)).max() <= 1e-4 * max(1.0, np.abs(np64(ud.grad)).max())
