@@ -37,6 +37,8 @@ void set_error(const char *fmt, ...);  // api.hip (thread-local buffer)
 
 static inline __host__ __device__ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline __host__ __device__ int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
+// The largest sizes.  N: four rows of code words lie within a 32-bit offset; gradients: eight rows of float32.
+constexpr int64_t MAX_MK = 1 << 30, MAX_N_W4 = 1 << 25, MAX_N_GRADS = 1 << 26;
 // A dimension of a launch holds fewer than 2^32 threads: a larger one runs as its remainder, without an error.
 static inline bool launchable(int64_t blocks, int threads) { return blocks < (int64_t(1) << 32) / threads; }
 static inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

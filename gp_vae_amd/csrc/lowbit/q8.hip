@@ -118,8 +118,8 @@ __global__ __launch_bounds__(256) void load_q8_kernel(int64_t M, int64_t K, cons
 
 static int check_q8(const char *fn, int dtype, int64_t M, int64_t K) {
   LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
-  LB_REQUIRE(M >= 0 && M <= (1 << 30), 3, "%s: M must lie in [0, 2^30] (got %lld)", fn, (long long)M);
-  LB_REQUIRE(K >= 1 && K <= (1 << 30), 4, "%s: K must lie in [1, 2^30] (got %lld)", fn, (long long)K);
+  LB_REQUIRE(M >= 0 && M <= MAX_MK, 3, "%s: M must lie in [0, 2^30] (got %lld)", fn, (long long)M);
+  LB_REQUIRE(K >= 1 && K <= MAX_MK, 4, "%s: K must lie in [1, 2^30] (got %lld)", fn, (long long)K);
   return 0;
 }
 
@@ -176,7 +176,7 @@ extern "C" int gpvae_load_q8(void *stream, int dtype, int64_t M, int64_t K, int 
 }
 
 extern "C" int64_t gpvae_dense_grads_q8_workspace_bytes(int dtype, int64_t M, int64_t K, int64_t N) {
-  if (!dtype_ok(dtype) || M < 0 || K < 1 || N < 1) return 0;
+  if (!dtype_ok(dtype) || M < 0 || M > MAX_MK || K < 1 || K > MAX_MK || N < 1 || N > MAX_N_GRADS) return 0;
   const GradsPlan p = grads_plan(pieces(dtype), M, K, N);
   return p.splits > 1 ? p.splits * (K + 1) * N * 4 : 0;
 }
@@ -186,7 +186,7 @@ extern "C" int gpvae_dense_grads_q8(void *stream, int dtype, int64_t M, int64_t 
                                     void *work) {
   const char *fn = "gpvae_dense_grads_q8";
   if (const int rc = check_q8(fn, dtype, M, K)) return rc;
-  LB_REQUIRE(N >= 1 && N <= (1 << 26), 5, "%s: N must lie in [1, 2^26] (got %lld)", fn, (long long)N);
+  LB_REQUIRE(N >= 1 && N <= MAX_N_GRADS, 5, "%s: N must lie in [1, 2^26] (got %lld)", fn, (long long)N);
   LB_REQUIRE(M == 0 || (codes && aligned16(codes)), 7, "%s: codes must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(M == 0 || (exps && aligned16(exps)), 8, "%s: exps must be a 16-byte aligned device pointer", fn);
   LB_REQUIRE(M == 0 || dY, 9, "%s: dY is NULL", fn);

@@ -91,9 +91,8 @@ __global__ __launch_bounds__(256) void load_w4_kernel(int64_t K, int64_t N, cons
 
 static int check_w4(const char *fn, int dtype, int64_t K, int64_t N, int kn_arg) {
   LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
-  // N: four rows of code words lie within a 32-bit offset
-  LB_REQUIRE(K >= 1 && K <= (1 << 30), kn_arg, "%s: K must lie in [1, 2^30] (got %lld)", fn, (long long)K);
-  LB_REQUIRE(N >= 1 && N <= (1 << 25), kn_arg + 1, "%s: N must lie in [1, 2^25] (got %lld)", fn, (long long)N);
+  LB_REQUIRE(K >= 1 && K <= MAX_MK, kn_arg, "%s: K must lie in [1, 2^30] (got %lld)", fn, (long long)K);
+  LB_REQUIRE(N >= 1 && N <= MAX_N_W4, kn_arg + 1, "%s: N must lie in [1, 2^25] (got %lld)", fn, (long long)N);
   return 0;
 }
 
@@ -163,7 +162,8 @@ static inline bool use_skinny(int P, int64_t M, int64_t L, int64_t O, bool vjp) 
   return groups <= 16 && work <= 3 * 0x1p30;
 }
 static int64_t w4_workspace(int dtype, int64_t M, int64_t L, int64_t O, bool vjp) {
-  if (!dtype_ok(dtype) || M < 1 || L < 1 || O < 1) return 0;
+  const int64_t K = vjp ? O : L, N = vjp ? L : O;
+  if (!dtype_ok(dtype) || M < 1 || M > MAX_MK || K < 1 || K > MAX_MK || N < 1 || N > MAX_N_W4) return 0;
   const int P = pieces(dtype);
   if (use_skinny(P, M, L, O, vjp)) {
     const SkinnyPlan p = skinny_plan(P, M, L, O);
@@ -208,7 +208,7 @@ extern "C" int gpvae_dense_w4(void *stream, int dtype, int64_t M, int64_t K, int
                               void *work) {
   const char *fn = "gpvae_dense_w4";
   LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
-  LB_REQUIRE(M >= 0 && M <= (1 << 30), 3, "%s: M must lie in [0, 2^30] (got %lld)", fn, (long long)M);
+  LB_REQUIRE(M >= 0 && M <= MAX_MK, 3, "%s: M must lie in [0, 2^30] (got %lld)", fn, (long long)M);
   if (const int rc = check_w4(fn, dtype, K, N, 4)) return rc;
   if (M == 0) return 0;
   LB_REQUIRE(X, 6, "%s: X is NULL", fn);
@@ -232,7 +232,7 @@ extern "C" int gpvae_dense_vjp_w4(void *stream, int dtype, int64_t M, int64_t K,
                                   void *work) {
   const char *fn = "gpvae_dense_vjp_w4";
   LB_REQUIRE(dtype_ok(dtype), 2, "%s: dtype must be float32, bfloat16 or float16 (got %d)", fn, dtype);
-  LB_REQUIRE(M >= 0 && M <= (1 << 30), 3, "%s: M must lie in [0, 2^30] (got %lld)", fn, (long long)M);
+  LB_REQUIRE(M >= 0 && M <= MAX_MK, 3, "%s: M must lie in [0, 2^30] (got %lld)", fn, (long long)M);
   if (const int rc = check_w4(fn, dtype, K, N, 4)) return rc;
   if (M == 0) return 0;
   LB_REQUIRE(dY, 6, "%s: dY is NULL", fn);

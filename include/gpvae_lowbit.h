@@ -47,7 +47,8 @@ const char *gpvae_lowbit_last_error(void);
 /* ---- w4: weights in 4 bits ------------------------------------------------------------------------------
  * gpvae_quant_w4   W [K, ldw] -> codes, exps: every value to the nearest of its tile's 15, ties to the even code.
  * gpvae_load_w4    the values W~ the codes stand for, out [K, ldo] (exact in float32 and bfloat16).
- * 1 <= K <= 2^30, 1 <= N <= 2^25 (here and in the products).                                               */
+ * 1 <= K <= 2^30, 1 <= N <= 2^25 (here and in the products; M up to 2^30 in every call).  A workspace query of sizes
+ * that its call refuses gives 0.                                                                            */
 int64_t gpvae_w4_code_bytes(int64_t K, int64_t N);
 int64_t gpvae_w4_exp_bytes(int64_t K, int64_t N);
 int gpvae_quant_w4(void *stream, int dtype, int64_t K, int64_t N, const void *W, int64_t ldw, void *codes, void *exps);

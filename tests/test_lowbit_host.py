@@ -164,3 +164,18 @@ def test_launches_hold_fewer_than_2_32_threads_in_a_dimension():
     for fn, k, n in ((lib.gpvae_dense_w4_workspace_bytes, 640, 50), (lib.gpvae_dense_vjp_w4_workspace_bytes, 50, 640)):
         for rows in (2 ** 24, 2 ** 24 + 70, 2 ** 30):
             assert fn(0, rows, k, n) == fn(0, 2 ** 20, k, n) == 3 * 2 ** 20 * 640 * 2
+
+
+def test_workspace_queries_of_sizes_the_calls_refuse():
+    lib = _lib.load_lowbit()
+    for big in (2 ** 30 + 1, 2 ** 31, 2 ** 32 * 128, 2 ** 38, 2 ** 40, 2 ** 62, 2 ** 63 - 1):
+        for name in ("gpvae_dense_w4_workspace_bytes", "gpvae_dense_vjp_w4_workspace_bytes", "gpvae_dense_grads_q8_workspace_bytes"):
+            fn = getattr(lib, name)
+            for dt in (0, 2, 3):
+                for at in range(3):
+                    sizes = [1000, 1000, 1000]
+                    sizes[at] = big
+                    assert fn(dt, *sizes) == 0, (name, dt, sizes)
+    assert lib.gpvae_dense_w4_workspace_bytes(0, 1000, 1000, 2 ** 25 + 1) == 0 and lib.gpvae_dense_vjp_w4_workspace_bytes(0, 1000, 1000, 2 ** 25 + 1) == 0
+    assert lib.gpvae_dense_grads_q8_workspace_bytes(0, 1000, 1000, 2 ** 26 + 1) == 0
+    assert lib.gpvae_dense_w4_workspace_bytes(0, 2 ** 30, 2 ** 30, 2 ** 25) > 0 and lib.gpvae_dense_vjp_w4_workspace_bytes(0, 2 ** 30, 2 ** 30, 2 ** 25) > 0
